@@ -143,7 +143,7 @@ def work(case):
     f = 6.0 * n * dk * dv
     if case['train']:
         b += size * n * (4 * dk + 3 * dv) + 4.0 * s * dk * dv * (
-            3 if case['state'] else 1)
+            3 if case['state'] else 0)
         f += 14.0 * n * dk * dv
     return dict(bytes=b, flops=f)
 
