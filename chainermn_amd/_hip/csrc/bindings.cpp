@@ -90,8 +90,51 @@ torch::Tensor bn_bwd_input(torch::Tensor x, torch::Tensor gy,
                            torch::Tensor gamma, torch::Tensor gbeta,
                            torch::Tensor ggamma, double total_count);
 
+torch::Tensor embed_id(torch::Tensor ids, torch::Tensor w, double scale,
+                       bool has_ignore, long ignore);
+torch::Tensor embed_lookup(torch::Tensor ids, torch::Tensor w, double scale,
+                           bool has_ignore, long ignore);
+torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
+                         double scale, bool has_ignore, long ignore);
+torch::Tensor dropout_fn(torch::Tensor x, torch::Tensor key, long threshold,
+                         double scale);
+torch::Tensor dropout_next_key(torch::Tensor state);
+std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor w,
+                                    c10::optional<torch::Tensor> res,
+                                    double eps);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fp8(
+    torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> res,
+    double eps, long group);
+std::vector<torch::Tensor> linear_attention(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v,
+    torch::Tensor log_decay, c10::optional<torch::Tensor> first,
+    c10::optional<torch::Tensor> lengths, double scale);
+torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
+                                    torch::Tensor v, torch::Tensor state,
+                                    torch::Tensor log_decay, double scale);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "chainermn_amd MI355X (gfx950) kernels";
+  m.def("embed_id", &embed_id, "scaled embedding lookup, differentiable",
+        py::call_guard<py::gil_scoped_release>());
+  m.def("embed_lookup", &embed_lookup, "scaled embedding lookup");
+  m.def("embed_grad", &embed_grad,
+        "dense gradient of the table by sorted tokens (no float atomics)");
+  m.def("dropout", &dropout_fn,
+        "dropout from Philox4x32-10, differentiable (no mask is stored)",
+        py::call_guard<py::gil_scoped_release>());
+  m.def("dropout_next_key", &dropout_next_key,
+        "(seed, call) for one dropout; the state's call number goes up");
+  m.def("rms_norm", &rms_norm,
+        "[y] or [y, x + residual], differentiable",
+        py::call_guard<py::gil_scoped_release>());
+  m.def("rms_norm_fp8", &rms_norm_fp8,
+        "(e4m3 output, scales, x + residual)");
+  m.def("linear_attention", &linear_attention,
+        "[o, last state] with a decay for each head, differentiable",
+        py::call_guard<py::gil_scoped_release>());
+  m.def("linear_attention_step", &linear_attention_step,
+        "one token; the state is updated in place");
   m.def("batched_pack", &batched_pack,
         "gather param grads into flat wire buffer (fused cast, K1)");
   m.def("batched_unpack", &batched_unpack,

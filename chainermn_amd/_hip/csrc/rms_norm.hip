@@ -1,0 +1,511 @@
+// Root-mean-square norm with the residual's addition.
+//
+//   h = x + residual            (rounded once where it is written)
+//   y = h * rstd * w,  rstd = 1 / sqrt(mean(h^2) + eps)
+//
+// and, with g = gy * w and xhat = h * rstd,
+//
+//   dh = rstd * (g - xhat * mean(g * xhat)) + gh,   dw = sum_rows gy * xhat.
+//
+// A row stays in registers: every input is read once and every output
+// written once, which bounds all three kernels.  y is computed from the
+// unrounded sum; the backward pass reads the rounded one, so its xhat is
+// off by half a step of the type.  Sums and rstd are fp32.
+//
+// A row belongs to `tpr` threads: a wave where it fits, or a workgroup.
+
+#include "seq_common.h"
+
+namespace {
+
+using namespace seq;
+
+constexpr int kMaxDim = 16384;
+
+// vectors of a row that a thread holds: 16 to 32 elements
+template <int VE>
+constexpr int kHeld = VE >= 4 ? 4 : VE == 2 ? 8 : 16;
+
+// The sum over the row's threads, for all of them.  `lds` holds one float
+// for each wave of the workgroup and is written again by the next call, so
+// that calls alternate between two of them.
+__device__ __forceinline__ float row_sum(float v, int tpr, float* lds) {
+  v = wave_sum(v);
+  if (tpr > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int base = threadIdx.x / tpr * (tpr >> 6);
+    v = 0.f;
+    for (int i = 0; i < tpr >> 6; ++i) v += lds[base + i];
+  }
+  return v;
+}
+
+__device__ __forceinline__ float row_max(float v, int tpr, float* lds) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    v = fmaxf(v, __shfl_xor(v, off, 64));
+  if (tpr > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int base = threadIdx.x / tpr * (tpr >> 6);
+    for (int i = 0; i < tpr >> 6; ++i) v = fmaxf(v, lds[base + i]);
+  }
+  return v;
+}
+
+template <typename T, int VE>
+__device__ __forceinline__ void load_weight(const void* w, bool w32, long c,
+                                            float (&r)[VE]) {
+  if (w32) load<float, VE>((const float*)w + c, r);
+  else load<T, VE>((const T*)w + c, r);
+}
+
+// h of a row and its rstd; the sum is written to `sum` if there is one.
+template <typename T, int VE>
+__device__ __forceinline__ float read_row(
+    const T* x, const T* res, T* sum, int dim, int t, int tpr, float eps,
+    float* lds, float (&h)[kHeld<VE>][VE]) {
+  float sq = 0.f;
+#pragma unroll
+  for (int k = 0; k < kHeld<VE>; ++k) {
+    const int c = (k * tpr + t) * VE;
+    if (c < dim) {
+      load<T, VE>(x + c, h[k]);
+      if (res) {
+        float r[VE];
+        load<T, VE>(res + c, r);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) h[k][i] += r[i];
+        store<T, VE>(sum + c, h[k]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) h[k][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) sq += h[k][i] * h[k][i];
+  }
+  return rsqrtf(row_sum(sq, tpr, lds) / dim + eps);
+}
+
+template <typename T, int VE>
+__global__ __launch_bounds__(1024) void rms_fwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ res,
+    const void* __restrict__ w, bool w32, T* __restrict__ y,
+    T* __restrict__ sum, float* __restrict__ rstd_out, long rows, int dim,
+    long xs, long rs, int tpr, float eps) {
+  __shared__ float lds[2][16];
+  const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
+  int turn = 0;
+  for (long r0 = blockIdx.x * (long)per; r0 < rows;
+       r0 += gridDim.x * (long)per, turn ^= 1) {
+    long row = r0 + threadIdx.x / tpr;
+    const bool on = row < rows;  // whole waves, and all of them at barriers
+    if (!on) row = rows - 1;
+    float h[kHeld<VE>][VE];
+    const float rstd = read_row<T, VE>(
+        x + row * xs, res ? res + row * rs : nullptr, sum + row * dim, dim, t,
+        tpr, eps, lds[turn], h);
+    if (!on) continue;
+    if (rstd_out && t == 0) rstd_out[row] = rstd;
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      if (c < dim) {
+        float wt[VE];
+        load_weight<T, VE>(w, w32, c, wt);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) h[k][i] = h[k][i] * rstd * wt[i];
+        store<T, VE>(y + row * dim + c, h[k]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float e4m3_scale(float amax) {
+  const float s = amax / 448.f;
+  return s > 0.f ? s : 1.f;  // a row of zeros
+}
+
+template <int VE>
+__device__ __forceinline__ void store_e4m3(unsigned char* p, float scale,
+                                           const float (&y)[VE]) {
+  float q[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const float v = y[i] / scale;
+    // comparisons keep NaN
+    q[i] = v > 448.f ? 448.f : v < -448.f ? -448.f : v;
+  }
+  if constexpr (VE >= 4) {
+    unsigned u[VE / 4];
+#pragma unroll
+    for (int i = 0; i < VE / 4; ++i) {
+      int b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0,
+                                              false);
+      b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], b,
+                                          true);
+      u[i] = b;
+    }
+    if constexpr (VE == 8)
+      *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    else
+      *reinterpret_cast<unsigned*>(p) = u[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[i], q[i], 0, false) & 0xff;
+  }
+}
+
+// y in e4m3 with a scale for each row (group = 0) or each `group` columns,
+// 2^n of them that at most a wave holds: amax / 448.
+template <typename T, int VE>
+__global__ __launch_bounds__(1024) void rms_fp8_kernel(
+    const T* __restrict__ x, const T* __restrict__ res,
+    const void* __restrict__ w, bool w32, unsigned char* __restrict__ q,
+    float* __restrict__ scales, T* __restrict__ sum, long rows, int dim,
+    long xs, long rs, int tpr, float eps, int group) {
+  __shared__ float lds[2][16];
+  __shared__ float top[2][16];
+  const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
+  int turn = 0;
+  for (long r0 = blockIdx.x * (long)per; r0 < rows;
+       r0 += gridDim.x * (long)per, turn ^= 1) {
+    long row = r0 + threadIdx.x / tpr;
+    const bool on = row < rows;
+    if (!on) row = rows - 1;
+    float h[kHeld<VE>][VE];
+    const float rstd = read_row<T, VE>(
+        x + row * xs, res ? res + row * rs : nullptr, sum + row * dim, dim, t,
+        tpr, eps, lds[turn], h);
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      float m = 0.f;
+      if (c < dim) {
+        float wt[VE];
+        load_weight<T, VE>(w, w32, c, wt);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          h[k][i] = h[k][i] * rstd * wt[i];
+          m = fmaxf(m, fabsf(h[k][i]));
+        }
+      }
+      if (group) {
+        for (int off = group / VE / 2; off > 0; off >>= 1)
+          m = fmaxf(m, __shfl_xor(m, off, 64));
+        if (c < dim && on) {
+          const float s = e4m3_scale(m);
+          if (c % group == 0) scales[row * (dim / group) + c / group] = s;
+          store_e4m3<VE>(q + row * dim + c, s, h[k]);
+        }
+      }
+      amax = fmaxf(amax, m);
+    }
+    if (group) continue;
+    const float s = e4m3_scale(row_max(amax, tpr, top[turn]));
+    if (!on) continue;
+    if (t == 0) scales[row] = s;
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      if (c < dim) store_e4m3<VE>(q + row * dim + c, s, h[k]);
+    }
+  }
+}
+
+// dh of all rows, and the sum of gy * xhat over the workgroup's rows in
+// part[workgroup]: a thread's columns are the same for each of its rows.
+template <typename T, int VE>
+__global__ __launch_bounds__(1024) void rms_bwd_kernel(
+    const T* __restrict__ gy, const T* __restrict__ h,
+    const T* __restrict__ gh, const void* __restrict__ w, bool w32,
+    const float* __restrict__ rstd_in, T* __restrict__ dh,
+    float* __restrict__ part, long rows, int dim, long hs, int tpr) {
+  extern __shared__ float cols[];  // [dim], where a wave has a row
+  __shared__ float lds[2][16];
+  const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
+  float dw[kHeld<VE>][VE];
+#pragma unroll
+  for (int k = 0; k < kHeld<VE>; ++k)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) dw[k][i] = 0.f;
+  int turn = 0;
+  for (long r0 = blockIdx.x * (long)per; r0 < rows;
+       r0 += gridDim.x * (long)per, turn ^= 1) {
+    long row = r0 + threadIdx.x / tpr;
+    const bool on = row < rows;
+    if (!on) row = rows - 1;
+    const float rstd = rstd_in[row];
+    float g[kHeld<VE>][VE], xh[kHeld<VE>][VE];
+    float dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      if (c < dim && on) {
+        float wt[VE];
+        load<T, VE>(gy + row * dim + c, g[k]);
+        load<T, VE>(h + row * hs + c, xh[k]);
+        load_weight<T, VE>(w, w32, c, wt);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          xh[k][i] *= rstd;
+          dw[k][i] += g[k][i] * xh[k][i];
+          g[k][i] *= wt[i];
+          dot += g[k][i] * xh[k][i];
+        }
+      }
+    }
+    const float mean = row_sum(dot, tpr, lds[turn]) / dim;
+    if (!on) continue;
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      if (c < dim) {
+        float add[VE];
+        if (gh) {
+          load<T, VE>(gh + row * dim + c, add);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) add[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          add[i] += rstd * (g[k][i] - xh[k][i] * mean);
+        store<T, VE>(dh + row * dim + c, add);
+      }
+    }
+  }
+  float* out = part + blockIdx.x * (long)dim;
+  if (per == 1) {
+#pragma unroll
+    for (int k = 0; k < kHeld<VE>; ++k) {
+      const int c = (k * tpr + t) * VE;
+      if (c < dim) store<float, VE>(out + c, dw[k]);
+    }
+    return;
+  }
+  for (int p = 0; p < per; ++p) {  // one row of threads after another
+    if (threadIdx.x / tpr == p) {
+#pragma unroll
+      for (int k = 0; k < kHeld<VE>; ++k) {
+        const int c = (k * tpr + t) * VE;
+        if (c < dim) {
+          if (p > 0) {
+            float a[VE];
+            load<float, VE>(cols + c, a);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) dw[k][i] += a[i];
+          }
+          store<float, VE>(p + 1 == per ? out + c : cols + c, dw[k]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// dw: 16 columns of a workgroup, 16 threads for each.
+template <typename W>
+__global__ __launch_bounds__(256) void rms_dw_kernel(
+    const float* __restrict__ part, W* __restrict__ dw, int parts, int dim) {
+  __shared__ float lds[16][17];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15);
+  const int r = threadIdx.x >> 4;
+  float acc = 0.f;
+  if (c < dim) {
+#pragma unroll 8
+    for (int p = r; p < parts; p += 16) acc += part[(long)p * dim + c];
+  }
+  lds[r][threadIdx.x & 15] = acc;
+  __syncthreads();
+  if (r != 0 || c >= dim) return;
+  for (int i = 1; i < 16; ++i) acc += lds[i][threadIdx.x];
+  dw[c] = W(acc);
+}
+
+struct Rows {
+  long rows;
+  int dim, ve, tpr, block;
+};
+
+void check_matrix(const torch::Tensor& t, const torch::Tensor& like,
+                  const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 2 &&
+              t.sizes() == like.sizes() &&
+              t.scalar_type() == like.scalar_type() &&
+              (t.stride(1) == 1 || t.size(1) == 1),
+              "rms_norm: ", what, " must be a matrix like x with contiguous "
+              "rows on its GPU");
+}
+
+void check_weight(const torch::Tensor& w, const torch::Tensor& x) {
+  TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.dim() == 1 &&
+              w.size(0) == x.size(1) && w.is_contiguous() &&
+              (w.scalar_type() == x.scalar_type() ||
+               w.scalar_type() == at::kFloat),
+              "rms_norm: the weight is a contiguous vector for the rows, of "
+              "their type or float32, on their GPU");
+}
+
+int narrower(int ve, const torch::Tensor& t) {
+  const int n = vector_width(t.data_ptr(), t.size(-1),
+                             t.dim() == 2 ? t.stride(0) : 0,
+                             t.element_size());
+  return n < ve ? n : ve;
+}
+
+// A weight of fp32 is read by vectors of as many elements as x, at 16 bytes.
+int weight_width(int ve, const torch::Tensor& w) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(w.data_ptr());
+  int n = ve;
+  while (n > 1) {
+    const uintptr_t bytes = n * w.element_size();
+    if (p % (bytes < 16 ? bytes : 16) == 0) break;
+    n /= 2;
+  }
+  return n;
+}
+
+Rows plan(long rows, long dim, int ve) {
+  TORCH_CHECK(dim >= 1 && dim <= kMaxDim, "rms_norm: rows of 1 to ", kMaxDim,
+              " elements, not ", dim);
+  const int held = ve >= 4 ? 4 : ve == 2 ? 8 : 16;
+  int tpr = 64;
+  while (tpr * ve * held < dim) tpr *= 4;
+  return Rows{rows, (int)dim, ve, tpr, tpr < 256 ? 256 : tpr};
+}
+
+int grid_of(const Rows& r, int most) {
+  const long per = r.block / r.tpr;
+  const long n = (r.rows + per - 1) / per;
+  return int(n < most ? n : most);
+}
+
+}  // namespace
+
+// (y, h, rstd): h is empty without a residual.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fwd(
+    torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> res,
+    double eps) {
+  check_matrix(x, x, "x");
+  check_weight(w, x);
+  const c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
+  int ve = weight_width(narrower(16 / (int)x.element_size(), x), w);
+  if (res) {
+    check_matrix(*res, x, "the residual");
+    ve = narrower(ve, *res);
+  }
+  const Rows r = plan(rows, dim, ve);
+  auto y = torch::empty({rows, dim}, x.options());
+  auto h = torch::empty({res ? rows : 0, dim}, x.options());
+  auto rstd = torch::empty({rows}, x.options().dtype(at::kFloat));
+  if (rows == 0) return {y, h, rstd};
+  dispatch_vec(x.scalar_type(), ve, "rms_norm", [&](auto t, auto width) {
+    using T = decltype(t);
+    constexpr int VE = decltype(width)::value;
+    rms_fwd_kernel<T, VE>
+        <<<dim3(grid_of(r, 4096)), dim3(r.block), 0, stream()>>>(
+            (const T*)x.data_ptr(), res ? (const T*)res->data_ptr() : nullptr,
+            w.data_ptr(), w.scalar_type() == at::kFloat, (T*)y.data_ptr(),
+            (T*)h.data_ptr(), rstd.data_ptr<float>(), rows, r.dim,
+            x.stride(0), res ? res->stride(0) : 0, r.tpr, (float)eps);
+  });
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {y, h, rstd};
+}
+
+// (q, scales, h): e4m3 with a scale for each row or each `group` columns.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fp8(
+    torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> res,
+    double eps, long group) {
+  check_matrix(x, x, "x");
+  check_weight(w, x);
+  const c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
+  const int full = 16 / (int)x.element_size();
+  int ve = weight_width(narrower(full, x), w);
+  if (res) {
+    check_matrix(*res, x, "the residual");
+    ve = narrower(ve, *res);
+  }
+  TORCH_CHECK(group == 0 || ((group & (group - 1)) == 0 && group >= 16 &&
+                             group <= 256 && dim % group == 0),
+              "rms_norm_fp8: groups of 16, 32, 64, 128 or 256 columns that "
+              "divide the row, not ", group);
+  // a group is joined inside of a wave
+  TORCH_CHECK(group <= 64 * ve, "rms_norm_fp8: rows that are not aligned to "
+              "16 bytes cannot take groups of ", group);
+  const Rows r = plan(rows, dim, ve);
+  auto q = torch::empty({rows, dim},
+                        x.options().dtype(at::kFloat8_e4m3fn));
+  auto scales = torch::empty({rows, group ? dim / group : 1},
+                             x.options().dtype(at::kFloat));
+  auto h = torch::empty({res ? rows : 0, dim}, x.options());
+  if (rows == 0) return {q, scales, h};
+  dispatch_vec(x.scalar_type(), ve, "rms_norm_fp8", [&](auto t, auto width) {
+    using T = decltype(t);
+    constexpr int VE = decltype(width)::value;
+    rms_fp8_kernel<T, VE>
+        <<<dim3(grid_of(r, 4096)), dim3(r.block), 0, stream()>>>(
+            (const T*)x.data_ptr(), res ? (const T*)res->data_ptr() : nullptr,
+            w.data_ptr(), w.scalar_type() == at::kFloat,
+            (unsigned char*)q.data_ptr(), scales.data_ptr<float>(),
+            (T*)h.data_ptr(), rows, r.dim, x.stride(0),
+            res ? res->stride(0) : 0, r.tpr, (float)eps, (int)group);
+  });
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {q, scales, h};
+}
+
+// (dh, dw): gy and gh are contiguous, h has contiguous rows.
+std::tuple<torch::Tensor, torch::Tensor> rms_norm_bwd(
+    torch::Tensor gy, torch::Tensor h, c10::optional<torch::Tensor> gh,
+    torch::Tensor w, torch::Tensor rstd) {
+  check_matrix(h, h, "h");
+  check_matrix(gy, h, "gy");
+  check_weight(w, h);
+  const c10::DeviceGuard guard(h.device());
+  const long rows = h.size(0), dim = h.size(1);
+  TORCH_CHECK(gy.is_contiguous() && rstd.is_cuda() &&
+              rstd.scalar_type() == at::kFloat && rstd.numel() == rows &&
+              rstd.is_contiguous(),
+              "rms_norm_bwd: gy contiguous, rstd float32 for each row");
+  int ve = weight_width(narrower(narrower(16 / (int)h.element_size(), h),
+                                 gy), w);
+  if (gh) {
+    check_matrix(*gh, h, "gh");
+    TORCH_CHECK(gh->is_contiguous(), "rms_norm_bwd: gh contiguous");
+    ve = narrower(ve, *gh);
+  }
+  const Rows r = plan(rows, dim, ve);
+  auto dh = torch::empty({rows, dim}, h.options());
+  auto dw = torch::empty({dim}, w.options());
+  const int grid = grid_of(r, 512);  // two of four waves on every CU
+  auto part = torch::empty({grid, dim}, h.options().dtype(at::kFloat));
+  if (rows) {
+    const int lds = r.block > r.tpr ? r.dim * (int)sizeof(float) : 0;
+    dispatch_vec(h.scalar_type(), ve, "rms_norm", [&](auto t, auto width) {
+      using T = decltype(t);
+      constexpr int VE = decltype(width)::value;
+      rms_bwd_kernel<T, VE><<<dim3(grid), dim3(r.block), lds, stream()>>>(
+          (const T*)gy.data_ptr(), (const T*)h.data_ptr(),
+          gh ? (const T*)gh->data_ptr() : nullptr, w.data_ptr(),
+          w.scalar_type() == at::kFloat, rstd.data_ptr<float>(),
+          (T*)dh.data_ptr(), part.data_ptr<float>(), rows, r.dim,
+          h.stride(0), r.tpr);
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  }
+  dispatch(w.scalar_type(), "rms_norm", [&](auto t) {
+    using W = decltype(t);
+    rms_dw_kernel<W><<<dim3((dim + 15) / 16), dim3(256), 0, stream()>>>(
+        part.data_ptr<float>(), (W*)dw.data_ptr(), grid, r.dim);
+  });
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {dh, dw};
+}

@@ -529,3 +529,10 @@ def gemm_nn_bnbwd(a, b, bnh):
         d = require().gemm_btw_bnbwd_bf16(a, bt, bx, mean, rstd, gamma,
                                           beta, partials)
     return d, partials
+
+
+# ---- sequence-model operators (their modules hold checks and CPU forms) ----
+
+from chainermn_amd.ops._dropout import dropout_next_key  # noqa: E402,F401
+from chainermn_amd.ops._linear_attention import linear_attention_step  # noqa: E402,F401,E501
+from chainermn_amd.ops._rms_norm import rms_norm_fp8  # noqa: E402,F401

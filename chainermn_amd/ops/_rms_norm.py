@@ -1,0 +1,91 @@
+"""Root-mean-square norm with the residual's addition: checks, the CPU form
+and the 8-bit output.
+
+Kernels: _hip/csrc/rms_norm.hip.
+"""
+
+import torch
+
+E4M3_MAX = 448.0
+MAX_DIM = 16384
+
+
+def check_rms_norm(x, weight, residual):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
+        raise ValueError('rms_norm: rows of 1 to {} elements, not {}'
+                         .format(MAX_DIM, tuple(x.shape)))
+    if weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+        raise ValueError('rms_norm: x is {}, the weight {}'.format(
+            tuple(x.shape), tuple(weight.shape)))
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError('rms_norm: x is {}, the weight {}'.format(
+            x.dtype, weight.dtype))
+    if residual is not None and (residual.shape != x.shape
+                                 or residual.dtype != x.dtype):
+        raise ValueError('rms_norm: x is {} {}, the residual {} {}'.format(
+            x.dtype, tuple(x.shape), residual.dtype, tuple(residual.shape)))
+    if weight.device != x.device or (residual is not None
+                                     and residual.device != x.device):
+        raise ValueError('rms_norm: x, weight and residual are on different '
+                         'devices')
+
+
+def rms_plain(x, weight, residual, eps):
+    """(y, h) in fp32 and not yet rounded."""
+    h = x.float()
+    if residual is not None:
+        h = h + residual.float()
+    y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
+    return y * weight.float(), h
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6, group=None):
+    """RMS norm with an output in 8 bits, for a product in e4m3.
+
+    Returns ``(q, scales)``, or ``(q, scales, x + residual)``: ``q`` is
+    float8_e4m3fn, ``q.float() * scale`` stands for the norm's output.  A
+    scale is the largest magnitude / 448 over a row (``scales`` is
+    ``[..., 1]``) or over ``group`` columns of it (``[..., dim / group]``;
+    16, 32, 64, 128 or 256 that divide the row), and 1 where all are zero.
+    Not differentiable.
+    """
+    check_rms_norm(x, weight, residual)
+    dim = x.shape[-1]
+    if group is not None and (group not in (16, 32, 64, 128, 256)
+                              or dim % group):
+        raise ValueError('rms_norm_fp8: groups of 16, 32, 64, 128 or 256 '
+                         'columns that divide the row of {}, not {}'
+                         .format(dim, group))
+    shape = x.shape
+    groups = dim // group if group else 1
+    if x.is_cuda:
+        from chainermn_amd import ops
+        m, r = _rows(x.detach()), None
+        if residual is not None:
+            r = _rows(residual.detach())
+        q, scales, h = ops.require().rms_norm_fp8(
+            m, weight.detach().contiguous(), r, float(eps), group or 0)
+        if x.dim() != 2:
+            q, scales = q.view(shape), scales.view(shape[:-1] + (groups,))
+            h = h.view(shape) if residual is not None else h
+        return (q, scales) if residual is None else (q, scales, h)
+    with torch.no_grad():
+        y, h = rms_plain(x, weight, residual, eps)
+        y = y.reshape(shape[:-1] + (groups, dim // groups))
+        scales = y.abs().amax(-1, keepdim=True) / E4M3_MAX
+        scales = torch.where(scales > 0, scales, torch.ones_like(scales))
+        q = (y / scales).clamp(-E4M3_MAX, E4M3_MAX)
+        q = q.to(torch.float8_e4m3fn).view(shape)
+        scales = scales.squeeze(-1)
+        return (q, scales) if residual is None else (q, scales,
+                                                     h.to(x.dtype))
+
+
+def _rows(x):
+    """A matrix of x's rows that can be read by 16 bytes if any copy can."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    size = x.element_size()
+    if x.stride(1) != 1 or x.stride(0) * size % 16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
