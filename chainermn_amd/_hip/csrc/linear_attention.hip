@@ -44,7 +44,8 @@ using frag = vec<bf16, 8>;
 using acc4 = vec<float, 4>;
 using half4 = vec<short, 4>;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of the kernels other than chunk_kernel
+constexpr int kChunk = 32;  // tokens
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Operand {
@@ -57,11 +58,10 @@ struct Role {
   void* out;           // [batch, length, heads, dv]
   const float* first;  // state that comes in, or null
   float* last;         // state that goes out, or null
-  float first_scale, last_scale;
   int dk, dv;          // of this role
-  bool state_by_v;     // the states' rows are this role's v index
+  float* states;       // [batch * heads][segments][D * D], in lane order
+  bool turned;         // states and ends are of the transposed state
   bool reverse;
-  bool wide;           // operands can be read by 16 bytes
   float intra, inter, gain;  // factors of scores, q S, and k^T v
 };
 
@@ -70,10 +70,30 @@ struct Problem {
   const float* log_decay;
   const void* lengths;  // or null
   bool long_lengths;
-  int batch, length, heads;
+  int batch, length, heads, roles;
   int segments, per_segment;  // tokens of a segment, a multiple of a chunk
-  float* states;  // [role][batch * heads][segments][D * D], in lane order
 };
+
+__device__ __forceinline__ long length_of(const Problem& pr, int b) {
+  if (!pr.lengths) return pr.length;
+  const long n = pr.long_lengths ? ((const long*)pr.lengths)[b]
+                                 : ((const int*)pr.lengths)[b];
+  return n < 0 ? 0 : n < pr.length ? n : pr.length;
+}
+
+// exp(-200) is zero in fp32, and 0 * log_decay has to be 0; NaN stays
+__device__ __forceinline__ float decay_of(const Problem& pr, int h) {
+  const float ld = pr.log_decay[h];
+  return ld < -200.f ? -200.f : ld;
+}
+
+// A buffer resource of `bytes`: reads behind it give zero, writes are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p,
+                                                         int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes,
+                                           0x00027000);
+}
+constexpr int kBehind = 0x7ffffff0;  // an offset behind any of them
 
 template <typename T>
 constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
@@ -81,14 +101,13 @@ template <>
 constexpr int kTerms<fp16> = 2;
 
 // Terms are cut off, not rounded: each is exact in bf16, and three of them
-// are the whole of an fp32.
+// are the whole of an fp32.  A term is the upper half of its word.
 template <int N>
 __device__ __forceinline__ void cut(float x, unsigned (&term)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const unsigned top = __float_as_uint(x) & 0xffff0000u;
-    term[i] = top;
-    if (i + 1 < N) x -= __uint_as_float(top);
+    term[i] = __float_as_uint(x);
+    if (i + 1 < N) x -= __uint_as_float(term[i] & 0xffff0000u);
   }
 }
 
@@ -97,47 +116,54 @@ __device__ __forceinline__ unsigned pair(unsigned a, unsigned b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302);
 }
 
-// A row-major tile of bf16 in LDS, rows of N elements.  Pieces of 32 bytes
-// are permuted within a row by the row's number, so that the 16 rows that a
-// fragment reads fall on all banks.
-template <int N>
-__device__ __forceinline__ int place(int row, int col) {
-  static_assert(N == 32 || N == 64 || N == 128, "row length");
-  constexpr int shift = N == 128 ? 0 : N == 64 ? 1 : 2;
-  constexpr int mask = N / 16 - 1;
-  return row * N + (col ^ (((row >> shift) & mask) << 4));
+// Tiles of bf16 in LDS are row-major with a padded pitch, so that every
+// fragment's address is a lane's base and a constant.  The pads put the eight
+// rows that are read at once on all banks: 32 bytes where a row gives 32 of
+// them (the transposing reads), 16 bytes where it gives 16.
+//
+// A tile whose rows are only read as fragments keeps its columns in the order
+// of the lanes: of 32 columns, 4g..4g+3 and 16+4g..16+4g+3 are neighbours.
+__device__ __forceinline__ int in_lane_order(int col) {
+  return (col & ~31) | ((col & 12) << 1) | ((col & 16) >> 2) | (col & 3);
 }
 
-// Fragment of 16 rows from `row`, 32 columns from `col`.
-template <int N>
+// Fragment of 16 rows from `row`, 32 columns from `col`, of a tile in lane
+// order.
+template <int PITCH>
 __device__ __forceinline__ frag by_row(const short* tile, int row, int col,
                                        int lane) {
-  const int r = row + (lane & 15), c = col + (lane >> 4) * 4;
+  return *reinterpret_cast<const frag*>(tile + (row + (lane & 15)) * PITCH +
+                                        col + (lane >> 4) * 8);
+}
+
+// The same of a tile in its own order.
+template <int PITCH>
+__device__ __forceinline__ frag by_row_plain(const short* tile, int row,
+                                             int col, int lane) {
+  const short* p = tile + (row + (lane & 15)) * PITCH + col + (lane >> 4) * 4;
   union {
     half4 h[2];
     frag f;
   } u;
-  u.h[0] = *reinterpret_cast<const half4*>(tile + place<N>(r, c));
-  u.h[1] = *reinterpret_cast<const half4*>(tile + place<N>(r, c + 16));
+  u.h[0] = *reinterpret_cast<const half4*>(p);
+  u.h[1] = *reinterpret_cast<const half4*>(p + 16);
   return u.f;
 }
 
 // Fragment of 16 columns from `col`, 32 rows from `row`: the transposing
 // read gives a lane four rows of one column.
-template <int N>
+template <int PITCH>
 __device__ __forceinline__ frag by_col(const short* tile, int row, int col,
                                        int lane) {
   using lds4 = __attribute__((address_space(3))) half4;
-  const int r = row + (lane >> 4) * 4 + ((lane & 15) >> 2);
-  const int c = col + (lane & 3) * 4;
+  const short* p = tile + (row + (lane >> 4) * 4 + ((lane & 15) >> 2)) *
+                              PITCH + col + (lane & 3) * 4;
   union {
     half4 h[2];
     frag f;
   } u;
-  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds4*)(tile + place<N>(r, c)));
-  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds4*)(tile + place<N>(r + 16, c)));
+  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * PITCH));
   return u.f;
 }
 
@@ -173,99 +199,155 @@ __device__ __forceinline__ void to_frag(const float (&x)[8], frag (&f)[N]) {
   for (int n = 0; n < N; ++n) f[n] = w[n].f;
 }
 
-// The rows of a chunk between global memory and LDS: a thread's part.
-template <typename T, int D, int C>
+// The rows of a chunk between global memory and LDS: a thread's part.  WIDE
+// operands are read by 16 bytes through a buffer resource that ends with the
+// last row, so that what lies behind it reads as zero without a branch.
+template <typename T, int D, int C, bool WIDE>
 struct Rows {
   static constexpr int VE = 16 / sizeof(T);
+  static constexpr int kThreads = D * 4;
   static constexpr int N = C * D / VE / kThreads;  // vectors of a thread
-  vec<T, VE> v[N];
+  static constexpr int kStep = kThreads / (D / VE);  // rows between them
+  union {
+    vec<T, VE> v[N];
+    vec<unsigned, 4> u[N];
+  };
 
   // rows at or behind `n` and columns at or behind `cols` are zero
   __device__ __forceinline__ void read(const T* p, long stride, int n,
-                                       int cols, bool wide) {
+                                       int cols) {
+    const int row = threadIdx.x / (D / VE);
+    const int col = threadIdx.x % (D / VE) * VE;
+    if constexpr (WIDE) {
+      const int pitch = int(stride * sizeof(T));
+      const int rows = n < C ? n : C;
+      const auto rsrc = buffer(p, (rows - 1) * pitch +
+                                      cols * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = i * kThreads + threadIdx.x;
-      const int row = at / (D / VE), col = at % (D / VE) * VE;
-      const T* src = p + row * stride + col;
-      if (wide) {
-        if (row < n && col < cols) {
-          v[i] = *reinterpret_cast<const vec<T, VE>*>(src);
-        } else {
+      for (int i = 0; i < N; ++i)
+        u[i] = __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, col < cols ? (row + i * kStep) * pitch +
+                                   col * (int)sizeof(T)
+                             : kBehind, 0, 0);
+    } else {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) v[i][e] = T(0.f);
-        }
-      } else {
+      for (int i = 0; i < N; ++i) {
+        const T* src = p + (row + i * kStep) * stride + col;
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-          v[i][e] = row < n && col + e < cols ? src[e] : T(0.f);
+          v[i][e] = row + i * kStep < n && col + e < cols ? src[e] : T(0.f);
       }
     }
   }
 
-  // planes of terms, each C * D
+  // planes of terms, each C * PITCH
+  template <int PITCH, bool LANE_ORDER>
   __device__ __forceinline__ void write(short* tile) const {
     constexpr int NT = kTerms<T>;
+    const int row = threadIdx.x / (D / VE);
+    const int col = threadIdx.x % (D / VE) * VE;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = i * kThreads + threadIdx.x;
-      const int row = at / (D / VE), col = at % (D / VE) * VE;
-      short* dst = tile + place<D>(row, col);
-      if constexpr (NT == 1) {
-        *reinterpret_cast<vec<T, VE>*>(dst) = v[i];
-      } else {
-        unsigned w[NT][VE / 2];
+      short* dst = tile + (row + i * kStep) * PITCH;
+      unsigned w[NT][VE / 2];
 #pragma unroll
-        for (int e = 0; e < VE; e += 2) {
+      for (int e = 0; e < VE; e += 2) {
+        if constexpr (NT == 1) {
+          w[0][e / 2] = u[i][e / 2];
+        } else {
           unsigned a[NT], b[NT];
           cut<NT>(float(v[i][e]), a);
           cut<NT>(float(v[i][e + 1]), b);
 #pragma unroll
           for (int n = 0; n < NT; ++n) w[n][e / 2] = pair(a[n], b[n]);
         }
+      }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if constexpr (VE == 8)
-            *reinterpret_cast<uint4*>(dst + n * C * D) =
-                make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]);
-          else
-            *reinterpret_cast<uint2*>(dst + n * C * D) =
-                make_uint2(w[n][0], w[n][1]);
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (VE == 8 && !LANE_ORDER) {
+          *reinterpret_cast<uint4*>(dst + n * C * PITCH + col) =
+              make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; e += 4)
+            *reinterpret_cast<uint2*>(
+                dst + n * C * PITCH +
+                (LANE_ORDER ? in_lane_order(col + e) : col + e)) =
+                make_uint2(w[n][e / 2], w[n][e / 2 + 1]);
         }
       }
     }
   }
 };
 
+// f(0), f(1) .. f(N - 1) with constants.
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>());
+  }
+}
+
 __device__ __forceinline__ float power(float log2, int n) {
   return __builtin_amdgcn_exp2f(log2 * n);
 }
 
+// LDS of a workgroup, in elements of 16 bits.
+template <typename T, int D>
+struct Lds {
+  static constexpr int C = kChunk;
+  static constexpr int NT = kTerms<T>, NI = NT == 3 ? 3 : 2;
+  static constexpr int kPitch = D + 16;                  // of k and v
+  // fp32 at 64 takes smaller pads and three workgroups fit into a CU
+  static constexpr int kPitchQ = D == 128 ? 176 : NT == 3 ? 72 : 80;
+  static constexpr int kPitchP = D == 64 && NT == 3 ? 40 : 48;
+  static constexpr int kTile = C * kPitch, kTileQ = C * kPitchQ;
+  static constexpr int kTileP = C * kPitchP;
+  static constexpr int kTables = 4 * C;                  // two of C floats
+  static constexpr int kState = kTables + 2 * NT * kTile;
+  static constexpr int kAll = kState + NT * kTileQ + NI * kTileP;
+};
+
+// Waves of a SIMD that registers have to leave room for: as many as LDS does.
+template <typename T, int D>
+constexpr int kWavesOfUnit = kTerms<T> < 3 ? 4 : D == 64 ? 3 : 2;
+
 // A workgroup takes a segment of a sequence and head for a role; a wave
-// keeps the state's columns of a quarter of dv.  OUT = false computes the
-// state of the segment alone.
-template <typename T, int D, int C, bool OUT>
-__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Problem pr) {
-  constexpr int NT = kTerms<T>;            // of the operands
-  constexpr int NI = NT == 3 ? 3 : 2;      // of scores and state, as operands
-  constexpr int LO = NT == 3 ? 2 : 1;      // terms that the output needs
+// keeps 16 columns of the state.  OUT = false computes the state of the
+// segment alone.
+template <typename T, int D, bool WIDE, bool OUT>
+__global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
+    Problem pr) {
+  using L = Lds<T, D>;
+  constexpr int C = kChunk;
+  constexpr int kThreads = D * 4, kWaves = D / 16;
+  constexpr int NT = L::NT;                // terms of the operands
+  constexpr int NI = L::NI;                // of scores and state, as operands
+  constexpr int LO = NT == 3 ? 2 : 1;      // that the output needs
   constexpr int KB = D / 32, KT = D / 16;  // blocks and tiles of dk
-  constexpr int W = D / 64;                // tiles of dv of a wave
-  constexpr int CT = C / 16, CB = C / 32;  // tiles and blocks of the chunk
-  constexpr int kTile = C * D;
+  constexpr int kTile = L::kTile, kTileQ = L::kTileQ, kTileP = L::kTileP;
 
   extern __shared__ __attribute__((aligned(16))) short lds[];
-  short* const kt = lds;
+  float* const gain = reinterpret_cast<float*>(lds);  // of a token in S
+  float* const seen = gain + C;                       // of S at a token
+  short* const kt = lds + L::kTables;
   short* const vt = kt + NT * kTile;
   short* const qt = vt + NT * kTile;
-  short* const pt = qt + (OUT ? NT * kTile : 0);  // scores, NI planes
+  short* const pt = qt + NT * kTileQ;
 
-  const Role& ro = pr.role[blockIdx.y];
+  // The roles of a problem follow each other on one XCD (workgroups go round
+  // the eight of them), where they share what they read in its L2.
+  const unsigned turn = blockIdx.x / (8 * pr.roles);
+  const unsigned in = blockIdx.x % (8 * pr.roles);
+  const unsigned id = turn * 8 + in % 8;
+  if (id >= (unsigned)pr.batch * pr.heads * pr.segments) return;
+  const Role& ro = pr.role[in / 8];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, l = lane & 15;
-  const int seg = blockIdx.x % pr.segments;
-  const int bh = blockIdx.x / pr.segments;
+  const int seg = id % pr.segments;
+  const int bh = id / pr.segments;
   const int b = bh / pr.heads, h = bh % pr.heads;
   const int dk = ro.dk, dv = ro.dv;
   const bool rev = ro.reverse;
@@ -273,111 +355,138 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Problem pr) {
   const int exit = rev ? 0 : pr.segments - 1;
   if (!OUT && seg == exit) return;  // nothing comes behind it
 
-  long len = pr.length;
-  if (pr.lengths) {
-    const long n = pr.long_lengths ? ((const long*)pr.lengths)[b]
-                                   : ((const int*)pr.lengths)[b];
-    len = n < 0 ? 0 : n < len ? n : len;
-  }
+  const long len = length_of(pr, b);
   const int seg0 = seg * pr.per_segment;
   const int seg1 = seg0 + pr.per_segment < pr.length
                        ? seg0 + pr.per_segment : pr.length;
   const int live = len < seg1 ? (len > seg0 ? int(len) - seg0 : 0)
                               : seg1 - seg0;  // tokens of the segment
   const int chunks = (live + C - 1) / C;
-
-  // exp(-200) is zero in fp32, and 0 * log2 has to be 0; NaN stays
-  float ld = pr.log_decay[h];
-  ld = ld < -200.f ? -200.f : ld;
+  const float ld = decay_of(pr, h);
   const float log2 = ld * kLog2e;
 
   const T* kp = (const T*)ro.k.p + b * ro.k.b + h * ro.k.h + seg0 * ro.k.t;
   const T* vp = (const T*)ro.v.p + b * ro.v.b + h * ro.v.h + seg0 * ro.v.t;
   const T* qp = (const T*)ro.q.p + b * ro.q.b + h * ro.q.h + seg0 * ro.q.t;
+  const long ostride = (long)pr.heads * dv;
   T* op = (T*)ro.out;
-  long ostride = 0;
-  if constexpr (OUT) {
-    ostride = (long)pr.heads * dv;
+  if constexpr (OUT)
     op += ((long)b * pr.length + seg0) * ostride + (long)h * dv;
-  }
 
-  // the state: tile t has rows 16t + 4g + r of dk, column l of dv tile w
-  acc4 s[KT][W];
-  float* mine = nullptr;
-  if (pr.states)
-    mine = pr.states + (((long)blockIdx.y * pr.batch * pr.heads + bh) *
-                            pr.segments + seg) * (D * D) + threadIdx.x * 4;
-  const int col0 = wave * W * 16;
+  // chunks on their way to LDS, in registers
+  constexpr int kAhead = OUT ? 1 : 2;
+  Rows<T, D, C, WIDE> kr[kAhead], vr[kAhead], qr[OUT ? kAhead : 1];
+  auto fetch = [&](int step, auto slot) {
+    if (step >= chunks) return;
+    constexpr int x = decltype(slot)::value;
+    const int t0 = (rev ? chunks - 1 - step : step) * C, n = live - t0;
+    kr[x].read(kp + t0 * ro.k.t, ro.k.t, n, dk);
+    vr[x].read(vp + t0 * ro.v.t, ro.v.t, n, dv);
+    if constexpr (OUT) qr[x].read(qp + t0 * ro.q.t, ro.q.t, n, dk);
+  };
+  each<kAhead>([&](auto slot) { fetch(slot, slot); });
+
+  // the state: tile t has rows 16t + 4g + r of dk, column col0 + l of dv
+  const int col0 = wave * 16;
+  acc4 s[KT];
   bool some = false;  // whether the state can be other than zero
+  float* stored = ro.states + ((long)bh * pr.segments + seg) * (D * D);
+  // byte offset of an element of an end's state
+  auto offset = [&](int i, int j) {
+    const int at = ro.turned ? j * dk + i : i * dv + j;
+    return i < dk && j < dv ? at * 4 : kBehind;
+  };
   if (seg == entry) {
     some = ro.first != nullptr;
+    const auto rsrc = buffer(ro.first + (some ? (long)bh * dk * dv : 0),
+                             some ? dk * dv * 4 : 0);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = t * 16 + 4 * g + r, j = col0 + w * 16 + l;
-          s[t][w][r] = some && i < dk && j < dv
-              ? ro.first[(long)bh * dk * dv +
-                         (ro.state_by_v ? (long)j * dk + i
-                                        : (long)i * dv + j)] * ro.first_scale
-              : 0.f;
-        }
-  } else if (OUT) {
+      for (int r = 0; r < 4; ++r)
+        s[t][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            rsrc, offset(t * 16 + 4 * g + r, col0 + l), 0, 0));
+  } else if constexpr (OUT) {
     some = true;
+    if (ro.turned) {  // stored for the transposed state: row and column swap
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        s[t][w] = *reinterpret_cast<const acc4*>(
-            mine + (t * W + w) * (kThreads * 4));
+        for (int r = 0; r < 4; ++r)
+          s[t][r] = stored[wave * (kThreads * 4) + t * 256 + (l >> 2) * 64 +
+                           (4 * g + r) * 4 + (l & 3)];
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+        s[t] = *reinterpret_cast<const acc4*>(stored + t * (kThreads * 4) +
+                                              threadIdx.x * 4);
+    }
   } else {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int w = 0; w < W; ++w) s[t][w] = acc4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < KT; ++t) s[t] = acc4{0.f, 0.f, 0.f, 0.f};
   }
 
-  Rows<T, D, C> kr, vr, qr;
-  auto fetch = [&](int c) {
-    const int t0 = c * C, n = live - t0;
-    kr.read(kp + t0 * ro.k.t, ro.k.t, n, dk, ro.wide);
-    vr.read(vp + t0 * ro.v.t, ro.v.t, n, dv, ro.wide);
-    if constexpr (OUT) qr.read(qp + t0 * ro.q.t, ro.q.t, n, dk, ro.wide);
-  };
-  if (chunks > 0) fetch(rev ? chunks - 1 : 0);
   if constexpr (OUT) {
-    // tiles of scores that the mask leaves empty are never written again
-    for (int i = threadIdx.x; i < NI * C * C / 2; i += kThreads)
+    // the tile of scores that the mask leaves empty is never written again
+    for (int i = threadIdx.x; i < NI * kTileP / 2; i += kThreads)
       reinterpret_cast<unsigned*>(pt)[i] = 0;
   }
 
-  for (int step = 0; step < chunks; ++step) {
+  auto decay_state = [&](float by) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        s[t][r] = __builtin_fmaf(s[t][r], by, s[t][r]);
+  };
+  if constexpr (!OUT) {
+    if (some) decay_state(expm1f(ld * live));
+  }
+  int of_tables = 0;   // the n that tables and `less` are for
+  float less = 0.f;    // lam^n - 1, which keeps a decay near one exact
+  auto chunk = [&](int step, auto slot) {
+    constexpr int x = decltype(slot)::value;
     const int c = rev ? chunks - 1 - step : step;
     const int n = live - c * C < C ? live - c * C : C;
     __syncthreads();  // the last chunk's readers are done
-    kr.write(kt);
-    vr.write(vt);
-    if constexpr (OUT) qr.write(qt);
-    if (step + 1 < chunks) fetch(rev ? c - 1 : c + 1);
+    if constexpr (!OUT) {
+      // alone, the state counts decays from the segment's end (backwards in
+      // time: from its beginning) and is not touched in between
+      const int i = threadIdx.x;
+      const int d = rev ? c * C + i + 1 : live - 1 - c * C - i;
+      if (i < C) gain[i] = ro.gain * power(log2, d > 0 ? d : 0);
+    } else if (n != of_tables) {  // the first chunk, and one not full
+      of_tables = n;
+      less = expm1f(ld * n);
+      const int i = threadIdx.x % C;
+      const int d = rev ? n - 1 - i : i + 1, e = rev ? i + 1 : n - 1 - i;
+      if (threadIdx.x < C) gain[i] = ro.gain * power(log2, e > 0 ? e : 0);
+      else if (threadIdx.x < 2 * C)
+        seen[i] = ro.inter * power(log2, d > 0 ? d : 0);
+    }
+    kr[x].template write<L::kPitch, false>(kt);
+    vr[x].template write<L::kPitch, false>(vt);
+    if constexpr (OUT) qr[x].template write<L::kPitchQ, true>(qt);
+    fetch(step + kAhead, slot);
     __syncthreads();
 
-    acc4 o[CT][W];
+    acc4 o[2] = {acc4{0.f, 0.f, 0.f, 0.f}, acc4{0.f, 0.f, 0.f, 0.f}};
     if constexpr (OUT) {
-      // scores, transposed: rows j, columns i
-      for (int e = wave; e < CT * (CT + 1) / 2; e += 4) {
-        const int hi = e < 1 ? 0 : e < 3 ? 1 : e < 6 ? 2 : 3;
-        const int lo = e - hi * (hi + 1) / 2;
-        const int it = rev ? lo : hi, jt = rev ? hi : lo;
+      // scores, transposed: rows j, columns i; the tiles (0, 0), (1, 1) and
+      // the one between them
+      if (wave < 3) {
+        const int it = rev ? wave == 1 : wave > 0;
+        const int jt = rev ? wave > 0 : wave == 1;
         acc4 p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           frag kf[NT], qf[NT];
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            kf[x] = by_row<D>(kt + x * kTile, jt * 16, kb * 32, lane);
-            qf[x] = by_row<D>(qt + x * kTile, it * 16, kb * 32, lane);
+            kf[x] = by_row_plain<L::kPitch>(kt + x * kTile, jt * 16, kb * 32,
+                                            lane);
+            qf[x] = by_row<L::kPitchQ>(qt + x * kTileQ, it * 16, kb * 32,
+                                       lane);
           }
           p = product<NT, NT, LO>(kf, qf, p);
         }
@@ -386,201 +495,184 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Problem pr) {
         for (int r = 0; r < 4; ++r) {
           const int i = it * 16 + l, j = jt * 16 + 4 * g + r;
           const int d = rev ? j - i : i - j;
-          const float x = d >= 0 ? p[r] * (ro.intra * power(log2, d)) : 0.f;
-          cut<NI>(x, term[r]);
+          cut<NI>(d >= 0 ? p[r] * (ro.intra * power(log2, d)) : 0.f, term[r]);
         }
 #pragma unroll
         for (int x = 0; x < NI; ++x)
           *reinterpret_cast<uint2*>(
-              pt + x * C * C + place<C>(it * 16 + l, jt * 16 + 4 * g)) =
+              pt + x * kTileP + (it * 16 + l) * L::kPitchP +
+              in_lane_order(jt * 16 + 4 * g)) =
               make_uint2(pair(term[0][x], term[1][x]),
                          pair(term[2][x], term[3][x]));
       }
 
       // q S, transposed: rows of dv, columns i
-#pragma unroll
-      for (int it = 0; it < CT; ++it)
-#pragma unroll
-        for (int w = 0; w < W; ++w) o[it][w] = acc4{0.f, 0.f, 0.f, 0.f};
       if (some) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          frag sf[W][NI];
+          float x[8];
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            float x[8];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[r] = s[2 * kb][w][r];
-              x[4 + r] = s[2 * kb + 1][w][r];
-            }
-            to_frag<NI>(x, sf[w]);
+          for (int r = 0; r < 4; ++r) {
+            x[r] = s[2 * kb][r];
+            x[4 + r] = s[2 * kb + 1][r];
           }
+          frag sf[NI];
+          to_frag<NI>(x, sf);
 #pragma unroll
-          for (int it = 0; it < CT; ++it) {
+          for (int it = 0; it < 2; ++it) {
             frag qf[NT];
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
-              qf[x] = by_row<D>(qt + x * kTile, it * 16, kb * 32, lane);
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-              o[it][w] = product<NI, NT, LO>(sf[w], qf, o[it][w]);
+            for (int y = 0; y < NT; ++y)
+              qf[y] = by_row<L::kPitchQ>(qt + y * kTileQ, it * 16, kb * 32,
+                                         lane);
+            o[it] = product<NI, NT, LO>(sf, qf, o[it]);
           }
         }
 #pragma unroll
-        for (int it = 0; it < CT; ++it) {
-          const int i = it * 16 + l;
-          const int d = rev ? n - 1 - i : i + 1;
-          const float f = ro.inter * power(log2, d > 0 ? d : 0);
-#pragma unroll
-          for (int w = 0; w < W; ++w) o[it][w] *= f;
-        }
+        for (int it = 0; it < 2; ++it) o[it] *= seen[it * 16 + l];
       }
       __syncthreads();  // the scores are whole
     }
 
-    const float less = expm1f(ld * n);  // keeps a decay near one exact
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          s[t][w][r] = __builtin_fmaf(s[t][w][r], less, s[t][w][r]);
+    if constexpr (OUT) {
+      decay_state(less);
+      some = true;
+    }
 
+    frag vf[NT], wf[3];  // v, and v with the weights of its tokens
 #pragma unroll
-    for (int jb = 0; jb < CB; ++jb) {
-      float weight[8];
+    for (int x = 0; x < NT; ++x)
+      vf[x] = by_col<L::kPitch>(vt + x * kTile, 0, col0, lane);
+    {
+      float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int j = jb * 32 + 4 * g + (e & 3) + (e >> 2) * 16;
-        const int d = rev ? j + 1 : n - 1 - j;
-        weight[e] = ro.gain * power(log2, d > 0 ? d : 0);
+        y[e] = float(vf[0][e]);
+#pragma unroll
+        for (int x = 1; x < NT; ++x) y[e] += float(vf[x][e]);
+        y[e] *= gain[(e >> 2) * 16 + 4 * g + (e & 3)];
       }
-      frag vf[W][NT], wf[W][3];
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-          vf[w][x] = by_col<D>(vt + x * kTile, jb * 32, col0 + w * 16, lane);
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          y[e] = float(vf[w][0][e]);
-#pragma unroll
-          for (int x = 1; x < NT; ++x) y[e] += float(vf[w][x][e]);
-          y[e] *= weight[e];
-        }
-        to_frag<3>(y, wf[w]);
-      }
-      if constexpr (OUT) {
-#pragma unroll
-        for (int it = 0; it < CT; ++it) {
-          if (rev ? it > 2 * jb + 1 : it < 2 * jb) continue;
-          frag pf[NI];
-#pragma unroll
-          for (int x = 0; x < NI; ++x)
-            pf[x] = by_row<C>(pt + x * C * C, it * 16, jb * 32, lane);
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            o[it][w] = product<NT, NI, LO>(vf[w], pf, o[it][w]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        frag kf[NT];
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-          kf[x] = by_col<D>(kt + x * kTile, jb * 32, t * 16, lane);
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-          s[t][w] = product<NT, 3, 2>(kf, wf[w], s[t][w]);
-      }
+      to_frag<3>(y, wf);
     }
-    some = true;
-
     if constexpr (OUT) {
 #pragma unroll
-      for (int it = 0; it < CT; ++it) {
-        const int i = it * 16 + l;
-        if (i >= n) continue;
+      for (int it = 0; it < 2; ++it) {
+        frag pf[NI];
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const int j = col0 + w * 16 + 4 * g;
+        for (int x = 0; x < NI; ++x)
+          pf[x] = by_row<L::kPitchP>(pt + x * kTileP, it * 16, 0, lane);
+        o[it] = product<NT, NI, LO>(vf, pf, o[it]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      frag kf[NT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+        kf[x] = by_col<L::kPitch>(kt + x * kTile, 0, t * 16, lane);
+      s[t] = product<NT, 3, 2>(kf, wf, s[t]);
+    }
+
+    if constexpr (OUT) {
+      const int j = col0 + 4 * g;
+      if constexpr (WIDE) {  // dv is a multiple of 4
+        const int pitch = int(ostride * sizeof(T));
+        const auto rsrc = buffer(op + c * C * ostride,
+                                 (n - 1) * pitch + dv * (int)sizeof(T));
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int at = j < dv ? (it * 16 + l) * pitch + j * (int)sizeof(T)
+                                : kBehind;
+          vec<T, 4> r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = T(o[it][e]);
+          if constexpr (sizeof(T) == 2)
+            __builtin_amdgcn_raw_buffer_store_b64(
+                __builtin_bit_cast(vec<unsigned, 2>, r), rsrc, at, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b128(
+                __builtin_bit_cast(vec<unsigned, 4>, r), rsrc, at, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int i = it * 16 + l;
+          if (i >= n) continue;
           T* dst = op + (c * C + i) * ostride + j;
-          float r[4] = {o[it][w][0], o[it][w][1], o[it][w][2], o[it][w][3]};
-          if (dv % 4 == 0) {
-            if (j < dv) store<T, 4>(dst, r);
-          } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (j + e < dv) dst[e] = T(r[e]);
-          }
+          for (int e = 0; e < 4; ++e)
+            if (j + e < dv) dst[e] = T(o[it][e]);
         }
       }
     }
-  }
+  };
+  for (int step = 0; step < chunks; step += kAhead)
+    each<kAhead>([&](auto slot) {
+      if (step + slot < chunks) chunk(step + slot, slot);
+    });
 
   if constexpr (OUT) {
     // behind the sequence's end the output is zero
-    for (int i = live + threadIdx.x / 64; i < seg1 - seg0; i += kThreads / 64)
+    for (int i = live + wave; i < seg1 - seg0; i += kWaves)
       for (int j = lane; j < dv; j += 64) op[i * ostride + j] = T(0.f);
     if (seg == exit && ro.last) {
+      const auto rsrc = buffer(ro.last + (long)bh * dk * dv, dk * dv * 4);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = t * 16 + 4 * g + r, j = col0 + w * 16 + l;
-            if (i < dk && j < dv)
-              ro.last[(long)bh * dk * dv +
-                      (ro.state_by_v ? (long)j * dk + i
-                                     : (long)i * dv + j)] =
-                  s[t][w][r] * ro.last_scale;
-          }
+        for (int r = 0; r < 4; ++r)
+          __builtin_amdgcn_raw_buffer_store_b32(
+              __float_as_uint(s[t][r]), rsrc,
+              offset(t * 16 + 4 * g + r, col0 + l), 0, 0);
     }
   } else {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-        *reinterpret_cast<acc4*>(mine + (t * W + w) * (kThreads * 4)) =
-            s[t][w];
+      *reinterpret_cast<acc4*>(stored + t * (kThreads * 4) +
+                               threadIdx.x * 4) = s[t];
   }
 }
 
-// The state of each segment alone becomes the state that comes into it.
-// grid: (elements / 1024, batch * heads, roles).
+// The state of each segment alone becomes the state that comes into it, for
+// the first role.  A thread has four elements of them all; the loads of 16
+// segments are in flight at once.  grid: (elements / 1024, batch * heads).
 __global__ __launch_bounds__(kThreads) void join_kernel(Problem pr,
                                                         int elements) {
-  const int bh = blockIdx.y, b = bh / pr.heads, h = bh % pr.heads;
-  const bool rev = pr.role[blockIdx.z].reverse;
-  long len = pr.length;
-  if (pr.lengths) {
-    const long n = pr.long_lengths ? ((const long*)pr.lengths)[b]
-                                   : ((const int*)pr.lengths)[b];
-    len = n < 0 ? 0 : n < len ? n : len;
-  }
-  float ld = pr.log_decay[h];
-  ld = ld < -200.f ? -200.f : ld;
-  float* p = pr.states +
-             ((long)blockIdx.z * gridDim.y + bh) * pr.segments * elements +
+  const int bh = blockIdx.y, b = bh / pr.heads;
+  const Role& ro = pr.role[0];
+  const long len = length_of(pr, b);
+  const float ld = decay_of(pr, bh % pr.heads);
+  float* p = ro.states + (long)bh * pr.segments * elements +
              (blockIdx.x * kThreads + threadIdx.x) * 4;
-  acc4 carry = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < pr.segments; ++i) {
-    const int seg = rev ? pr.segments - 1 - i : i;
-    acc4* at = reinterpret_cast<acc4*>(p + (long)seg * elements);
-    // the entry's own state holds what came in; the exit's is not computed
-    const acc4 own = i + 1 < pr.segments ? *at : carry;
-    if (i > 0) *at = carry;
-    const long left = len - (long)seg * pr.per_segment;
-    const int n = left < 0 ? 0
-                  : left < pr.per_segment ? int(left) : pr.per_segment;
-    const float less = expm1f(ld * n);
+  acc4 carry = {};
+  int of = -1;
+  float less = 0.f;
+  constexpr int U = 16;
+  for (int i0 = 0; i0 < pr.segments; i0 += U) {
+    acc4 own[U];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      carry[r] = __builtin_fmaf(carry[r], less, carry[r]) + own[r];
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u < pr.segments ? i0 + u : pr.segments - 1;
+      const int seg = ro.reverse ? pr.segments - 1 - i : i;
+      own[u] = *reinterpret_cast<const acc4*>(p + (long)seg * elements);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u, seg = ro.reverse ? pr.segments - 1 - i : i;
+      if (i < pr.segments) {
+        // the entry's own state holds what came in; the exit's is not
+        // computed, nor used
+        if (i > 0) *reinterpret_cast<acc4*>(p + (long)seg * elements) = carry;
+        const long left = len - (long)seg * pr.per_segment;
+        const int n = left < 0 ? 0
+                      : left < pr.per_segment ? int(left) : pr.per_segment;
+        if (n != of) less = expm1f(ld * n);
+        of = n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          carry[r] = __builtin_fmaf(carry[r], less, carry[r]) + own[u][r];
+      }
+    }
   }
 }
 
@@ -679,54 +771,93 @@ torch::Tensor rows_of(const torch::Tensor& x) {
   return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous();
 }
 
+// Whether rows can be read by 16 bytes through a buffer resource: aligned,
+// not on top of each other, and a chunk of them (and of the output) within
+// 2^30 bytes.
 bool is_wide(const torch::Tensor& x) {
   const int ve = 16 / (int)x.element_size();
   bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
             x.size(-1) % ve == 0;
   for (int i = 0; i + 1 < x.dim(); ++i)
     ok = ok && (x.size(i) == 1 || x.stride(i) % ve == 0);
-  return ok;
+  return ok && x.size(2) * x.size(3) < (1l << 21) &&
+         (x.size(1) == 1 || (x.stride(1) >= x.size(-1) &&
+                             x.stride(1) < (1l << 21)));
 }
 
 Operand operand(const torch::Tensor& x) {
-  return Operand{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)};
+  // the stride of an axis of one element can be anything
+  return Operand{x.data_ptr(), x.stride(0),
+                 x.size(1) == 1 ? x.size(3) : x.stride(1), x.stride(2)};
 }
 
-template <typename T, int D, int C>
-void run_chunks(Problem& pr, int roles) {
-  constexpr int NT = kTerms<T>, NI = NT == 3 ? 3 : 2;
-  const int lds_out = (3 * NT * C * D + NI * C * C) * 2;
-  const int lds_state = 2 * NT * C * D * 2;
-  const dim3 grid(pr.batch * pr.heads * pr.segments, roles);
-  if (pr.segments > 1) {
-    chunk_kernel<T, D, C, false>
-        <<<grid, dim3(kThreads), lds_state, stream()>>>(pr);
-    C10_HIP_KERNEL_LAUNCH_CHECK();
-    join_kernel<<<dim3(D * D / (kThreads * 4), pr.batch * pr.heads, roles),
-                  dim3(kThreads), 0, stream()>>>(pr, D * D);
-    C10_HIP_KERNEL_LAUNCH_CHECK();
+// The lengths of segments: 4 chunks and more, as long as all of them run at
+// once, two workgroups on each of 256 CUs.  A call and its backward pass cut
+// alike.
+struct Cut {
+  int d, segments, per_segment;
+  Cut(const torch::Tensor& q, const torch::Tensor& v) {
+    d = q.size(3) <= 64 && v.size(3) <= 64 ? 64 : 128;
+    const long alone = q.size(0) * q.size(2);
+    const long chunks = (q.size(1) + kChunk - 1) / kChunk;
+    const long n = std::max(1l, std::min(512 / alone, chunks / 4));
+    const long per = std::max(1l, (chunks + n - 1) / n);
+    per_segment = int(per * kChunk);
+    segments = std::max(1, int((chunks + per - 1) / per));
   }
-  auto kernel = chunk_kernel<T, D, C, true>;
-  // above 64 KB a workgroup has to ask
-  C10_HIP_CHECK(hipFuncSetAttribute(
-      (const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-      lds_out));
-  kernel<<<grid, dim3(kThreads), lds_out, stream()>>>(pr);
+  long states(const torch::Tensor& q) const {
+    return segments > 1 ? q.size(0) * q.size(2) * segments * d * d : 0;
+  }
+};
+
+template <typename T, int D, bool WIDE>
+void run_chunks(const Problem& pr, bool state) {
+  const long problems = (long)pr.batch * pr.heads * pr.segments;
+  const dim3 grid((problems + 7) / 8 * 8 * pr.roles);
+  if (state) {
+    chunk_kernel<T, D, WIDE, false>
+        <<<grid, dim3(D * 4), Lds<T, D>::kState * 2, stream()>>>(pr);
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    join_kernel<<<dim3(D * D / (kThreads * 4), pr.batch * pr.heads),
+                  dim3(kThreads), 0, stream()>>>(pr, D * D);
+  } else {
+    constexpr int lds = Lds<T, D>::kAll * 2;
+    auto kernel = chunk_kernel<T, D, WIDE, true>;
+    // above 64 KB a workgroup has to ask
+    if (lds > 65536)
+      C10_HIP_CHECK(hipFuncSetAttribute(
+          (const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+          lds));
+    kernel<<<grid, dim3(D * 4), lds, stream()>>>(pr);
+  }
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-void run_roles(Problem& pr, int roles, const torch::Tensor& q,
-               const torch::Tensor& log_decay,
-               const c10::optional<torch::Tensor>& lengths) {
+// The states of the first role's segments where `state`, and otherwise the
+// outputs of all roles.
+void run_roles(const Problem& pr, const Cut& cut, bool wide, at::ScalarType t,
+               bool state) {
+  dispatch(t, "linear_attention", [&](auto x) {
+    using T = decltype(x);
+    if (cut.d == 64 && wide) run_chunks<T, 64, true>(pr, state);
+    else if (cut.d == 64) run_chunks<T, 64, false>(pr, state);
+    else if (wide) run_chunks<T, 128, true>(pr, state);
+    else run_chunks<T, 128, false>(pr, state);
+  });
+}
+
+Problem problem(const torch::Tensor& q, const torch::Tensor& log_decay,
+                const c10::optional<torch::Tensor>& lengths, const Cut& cut) {
+  Problem pr{};
+  TORCH_CHECK(q.size(1) < (1l << 30) && q.size(0) * q.size(2) < (1l << 28),
+              "linear_attention: fewer than 2^30 tokens of a sequence and "
+              "2^28 sequences times heads");
   pr.batch = (int)q.size(0);
   pr.length = (int)q.size(1);
   pr.heads = (int)q.size(2);
-  TORCH_CHECK(q.size(1) < (1l << 30) && q.size(0) * q.size(2) < (1l << 30),
-              "linear_attention: fewer than 2^30 tokens of a sequence, and "
-              "sequences times heads");
+  pr.segments = cut.segments;
+  pr.per_segment = cut.per_segment;
   pr.log_decay = log_decay.data_ptr<float>();
-  pr.lengths = nullptr;
-  pr.long_lengths = false;
   if (lengths) {
     TORCH_CHECK(lengths->is_cuda() && lengths->device() == q.device() &&
                 lengths->dim() == 1 && lengths->size(0) == q.size(0) &&
@@ -738,44 +869,15 @@ void run_roles(Problem& pr, int roles, const torch::Tensor& q,
     pr.lengths = lengths->data_ptr();
     pr.long_lengths = lengths->scalar_type() == at::kLong;
   }
-  int widest = 0;
-  for (int i = 0; i < roles; ++i) {
-    widest = std::max(widest, std::max(pr.role[i].dk, pr.role[i].dv));
-  }
-  const int d = widest <= 64 ? 64 : 128;
-  const bool is_bf16 = q.scalar_type() == at::kBFloat16;
-  const int chunk = is_bf16 ? 64 : 32;
-  // Segments of 4 chunks and more, until two workgroups have work on each
-  // of 256 CUs.
-  const long alone = (long)pr.batch * pr.heads * roles;
-  const long chunks = (pr.length + chunk - 1) / chunk;
-  long segments = std::min((512 + alone - 1) / alone, chunks / 4);
-  if (segments < 1) segments = 1;
-  const long per = std::max(1l, (chunks + segments - 1) / segments);
-  pr.per_segment = int(per * chunk);
-  pr.segments = int((chunks + per - 1) / per);
-  if (pr.segments < 1) pr.segments = 1;
-  torch::Tensor space;
-  pr.states = nullptr;
-  if (pr.segments > 1) {
-    space = torch::empty({alone * pr.segments * d * d},
-                         q.options().dtype(at::kFloat));
-    pr.states = space.data_ptr<float>();
-  }
-  dispatch(q.scalar_type(), "linear_attention", [&](auto t) {
-    using T = decltype(t);
-    constexpr int C = sizeof(T) == 2 && std::is_same<T, bf16>::value ? 64
-                                                                     : 32;
-    if (d == 64) run_chunks<T, 64, C>(pr, roles);
-    else run_chunks<T, 128, C>(pr, roles);
-  });
+  return pr;
 }
 
 }  // namespace
 
-// (o, the state behind the sequence) of q, k [batch, length, heads, dk] and
-// v [batch, length, heads, dv].
-std::tuple<torch::Tensor, torch::Tensor> linear_attention_fwd(
+// (o, the state behind the sequences, the states before their segments) of
+// q, k [batch, length, heads, dk] and v [batch, length, heads, dv].  The
+// segments' states are for the backward pass, at most 512 of them.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
     torch::Tensor q, torch::Tensor k, torch::Tensor v,
     torch::Tensor log_decay, c10::optional<torch::Tensor> first,
     c10::optional<torch::Tensor> lengths, double scale) {
@@ -791,10 +893,14 @@ std::tuple<torch::Tensor, torch::Tensor> linear_attention_fwd(
   q = rows_of(q);
   k = rows_of(k);
   v = rows_of(v);
+  const auto floats = q.options().dtype(at::kFloat);
   auto o = torch::empty({b, q.size(1), h, dv}, q.options());
-  auto last = torch::empty({b, h, dk, dv}, q.options().dtype(at::kFloat));
-  if (last.numel() == 0) return {o, last};
-  Problem pr{};
+  auto last = torch::empty({b, h, dk, dv}, floats);
+  if (b * h == 0) return {o, last, torch::empty({0}, floats)};
+  const Cut cut(q, v);
+  auto states = torch::empty({cut.states(q)}, floats);
+  Problem pr = problem(q, log_decay, lengths, cut);
+  pr.roles = 1;
   Role& r = pr.role[0];
   r.q = operand(q);
   r.k = operand(k);
@@ -802,14 +908,15 @@ std::tuple<torch::Tensor, torch::Tensor> linear_attention_fwd(
   r.out = o.data_ptr();
   r.first = first ? first->data_ptr<float>() : nullptr;
   r.last = last.data_ptr<float>();
-  r.first_scale = r.last_scale = 1.f;
+  r.states = states.data_ptr<float>();
   r.dk = (int)dk;
   r.dv = (int)dv;
-  r.wide = is_wide(q) && is_wide(k) && is_wide(v);
   r.intra = r.inter = (float)scale;
   r.gain = 1.f;
-  run_roles(pr, 1, q, log_decay, lengths);
-  return {o, last};
+  const bool wide = is_wide(q) && is_wide(k) && is_wide(v);
+  if (cut.segments > 1) run_roles(pr, cut, wide, q.scalar_type(), true);
+  run_roles(pr, cut, wide, q.scalar_type(), false);
+  return {o, last, states};
 }
 
 // (dq, dk, dv, dfirst) of the gradients of o and of the last state; dfirst
@@ -819,7 +926,8 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                      torch::Tensor log_decay,
                      c10::optional<torch::Tensor> first,
                      c10::optional<torch::Tensor> lengths, double scale,
-                     torch::Tensor go, c10::optional<torch::Tensor> glast) {
+                     torch::Tensor states, torch::Tensor go,
+                     c10::optional<torch::Tensor> glast) {
   check_operand(q, q, 4, "q");
   check_operand(k, q, 4, "k");
   check_operand(v, q, 4, "v");
@@ -835,58 +943,60 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   k = rows_of(k);
   v = rows_of(v);
   go = rows_of(go);
+  const auto floats = q.options().dtype(at::kFloat);
   auto gq = torch::empty(q.sizes(), q.options());
   auto gk = torch::empty(k.sizes(), k.options());
   auto gv = torch::empty(v.sizes(), v.options());
-  auto gfirst = torch::empty({first ? b : 0, h, dk, dv},
-                             q.options().dtype(at::kFloat));
+  auto gfirst = torch::empty({first ? b : 0, h, dk, dv}, floats);
   if (b * h == 0) return {gq, gk, gv, gfirst};
-  Problem pr{};
+  const Cut cut(q, v);
+  TORCH_CHECK(states.numel() == cut.states(q) && states.is_contiguous() &&
+              states.device() == q.device() &&
+              states.scalar_type() == at::kFloat,
+              "linear_attention: states of another call");
+  auto gstates = torch::empty({cut.states(q)}, floats);
   const bool wide = is_wide(q) && is_wide(k) && is_wide(v) && is_wide(go);
   const float c = (float)scale;
-  Role& a = pr.role[0];  // dq = c do S^T
-  a.q = operand(go);
-  a.k = operand(v);
-  a.v = operand(k);
-  a.out = gq.data_ptr();
-  a.first = first ? first->data_ptr<float>() : nullptr;
-  a.first_scale = 1.f;
-  a.dk = (int)dv;
-  a.dv = (int)dk;
-  a.state_by_v = true;
-  a.wide = wide;
-  a.intra = a.inter = c;
-  a.gain = 1.f;
-  Role& e = pr.role[1];  // dv = k G
+  Problem pr = problem(q, log_decay, lengths, cut);
+  Role e{};  // dv = k G
   e.q = operand(k);
   e.k = operand(q);
   e.v = operand(go);
   e.out = gv.data_ptr();
   e.first = glast ? glast->data_ptr<float>() : nullptr;
-  e.first_scale = 1.f;
   e.last = first ? gfirst.data_ptr<float>() : nullptr;
-  e.last_scale = 1.f;
+  e.states = gstates.data_ptr<float>();
   e.dk = (int)dk;
   e.dv = (int)dv;
   e.reverse = true;
-  e.wide = wide;
   e.intra = e.gain = c;
   e.inter = 1.f;
-  Role& f = pr.role[2];  // dk = v G^T
+  Role f = e;  // dk = v G^T
   f.q = operand(v);
   f.k = operand(go);
   f.v = operand(q);
   f.out = gk.data_ptr();
-  f.first = e.first;
-  f.first_scale = 1.f;
+  f.last = nullptr;
   f.dk = (int)dv;
   f.dv = (int)dk;
-  f.state_by_v = true;
-  f.reverse = true;
-  f.wide = wide;
-  f.intra = f.gain = c;
-  f.inter = 1.f;
-  run_roles(pr, 3, q, log_decay, lengths);
+  f.turned = true;
+  Role a = f;  // dq = c do S^T
+  a.q = operand(go);
+  a.k = operand(v);
+  a.v = operand(k);
+  a.out = gq.data_ptr();
+  a.first = first ? first->data_ptr<float>() : nullptr;
+  a.states = states.data_ptr<float>();
+  a.reverse = false;
+  a.inter = c;
+  a.gain = 1.f;
+  pr.roles = 1;
+  pr.role[0] = e;
+  if (cut.segments > 1) run_roles(pr, cut, wide, q.scalar_type(), true);
+  pr.roles = 3;
+  pr.role[1] = f;
+  pr.role[2] = a;
+  run_roles(pr, cut, wide, q.scalar_type(), false);
   return {gq, gk, gv, gfirst};
 }
 

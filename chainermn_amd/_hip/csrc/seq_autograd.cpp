@@ -20,7 +20,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fwd(
 std::tuple<torch::Tensor, torch::Tensor> rms_norm_bwd(
     torch::Tensor gy, torch::Tensor h, c10::optional<torch::Tensor> gh,
     torch::Tensor w, torch::Tensor rstd);
-std::tuple<torch::Tensor, torch::Tensor> linear_attention_fwd(
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
     torch::Tensor q, torch::Tensor k, torch::Tensor v,
     torch::Tensor log_decay, c10::optional<torch::Tensor> first,
     c10::optional<torch::Tensor> lengths, double scale);
@@ -29,7 +29,8 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                      torch::Tensor log_decay,
                      c10::optional<torch::Tensor> first,
                      c10::optional<torch::Tensor> lengths, double scale,
-                     torch::Tensor go, c10::optional<torch::Tensor> glast);
+                     torch::Tensor states, torch::Tensor go,
+                     c10::optional<torch::Tensor> glast);
 
 namespace {
 
@@ -129,11 +130,11 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
                                c10::optional<Tensor> first,
                                c10::optional<Tensor> lengths, double scale) {
     ctx->set_materialize_grads(false);
-    auto [o, last] =
+    auto [o, last, states] =
         linear_attention_fwd(q, k, v, log_decay, first, lengths, scale);
     ctx->save_for_backward({q, k, v, log_decay,
                             first ? *first : Tensor(),
-                            lengths ? *lengths : Tensor()});
+                            lengths ? *lengths : Tensor(), states});
     ctx->saved_data["scale"] = scale;
     return {o, last};
   }
@@ -145,7 +146,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     const Tensor go = g[0].defined() ? g[0] : at::zeros_like(s[2]);
     auto [gq, gk, gv, gfirst] = linear_attention_bwd(
         s[0], s[1], s[2], s[3], some(s[4]), some(s[5]),
-        ctx->saved_data["scale"].toDouble(), go,
+        ctx->saved_data["scale"].toDouble(), s[6], go,
         g[1].defined() ? c10::optional<Tensor>(g[1].contiguous())
                        : c10::nullopt);
     return {gq, gk, gv, none, s[4].defined() ? gfirst : none, none, none};

@@ -21,7 +21,7 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None,
 
     Returns ``(o, state)``: ``o`` like v, and the fp32 state behind the
     sequences.  States and sums are fp32 whatever the type of q.  A value
-    that is not finite spreads to the outputs of its own chunk of 64 tokens,
+    that is not finite spreads to the outputs of its own chunk of 32 tokens,
     those before it included.
     """
     check_attention(q, k, v, log_decay, 4)
