@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(
         r[4 * h + j] = word[j] >= threshold ? r[4 * h + j] * scale : 0.f;
     }
     if (whole) {
-      store<T, 8>(y + i, r);
+      store<T, 8, true>(y + i, r);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -101,7 +101,9 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor key, long threshold,
   if (n == 0) return y;
   const bool aligned = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   long blocks = (n + 2047) / 2048;
-  if (blocks > 65536) blocks = 65536;  // the rest by strides of the grid
+  // the rest by strides of the grid (2^27 elements of bf16, both passes: 207
+  // us; with a workgroup for every 2048, 218 us)
+  if (blocks > 8192) blocks = 8192;
   dispatch(x.scalar_type(), "dropout", [&](auto t) {
     using T = decltype(t);
     dropout_kernel<T><<<dim3(blocks), dim3(256), 0, stream()>>>(

@@ -6,11 +6,13 @@
 // Both are bound by memory.  The gradient is three launches without float
 // atomics, so that its sums have one order and two runs agree bit by bit:
 //
-//   1. embed_sort: counting sort of the tokens by id.  A workgroup owns a
-//      range of at most 1024 ids and reads ALL ids (they come from L2): what
-//      it counts below its range is its place in the sorted order, so no
-//      workgroup waits for another one.
-//   2. embed_rows: a wave sums 32 sorted tokens of a slice of columns; rows
+//   1. embed_split and embed_sort: a stable counting sort of the tokens by
+//      id, first 1024 tokens of a workgroup by the low bits of their ids,
+//      then each of these buckets by the others.  A bucket's workgroup finds
+//      its place in the order from the counts of all of them, so none waits
+//      for another one.  Low bits, because the frequent words of a vocabulary
+//      sorted by frequency are neighbours.
+//   2. embed_rows: a wave sums 8 to 32 sorted tokens of some columns; rows
 //      that begin and end within its tokens are finished, the two at its
 //      ends leave partial sums.  So a frequent word costs no more than
 //      others.  Rows without a token are zeroed by further waves.
@@ -22,11 +24,19 @@ namespace {
 
 using namespace seq;
 
-constexpr int kSortThreads = 1024;
-constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kMaxBins = 1024;  // ids of a workgroup: 64 KB of counters
-constexpr int kChunk = 32;      // sorted tokens of a wave
+constexpr int kSplitThreads = 1024, kSplitWaves = kSplitThreads / 64;
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kMaxBins = 1024;    // ids of a workgroup of embed_sort
+constexpr int kMaxPieces = 1024;  // workgroups of embed_split
 constexpr int kJoinWaves = 8;
+
+// The column at which a lane reads and writes: the last vector of a row of
+// odd length is moved back onto the one before it, and both lanes compute the
+// same.  Rows shorter than a vector are read by elements.
+template <int VE>
+__device__ __forceinline__ long column(long c, long dim) {
+  return c + VE <= dim ? c : dim < VE ? 0 : dim - VE;
+}
 
 // ids behind this are neither looked up nor summed
 template <typename I>
@@ -36,33 +46,42 @@ __device__ __forceinline__ long id_at(const I* ids, long t, long vocab,
   return (id < 0 || id >= vocab || (has_ignore && id == ignore)) ? -1 : id;
 }
 
-template <typename T, int VE, typename I>
+template <typename T, typename I>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(
     const I* __restrict__ ids, const T* __restrict__ w, T* __restrict__ y,
     long n, long vocab, long dim, long stride, float scale, bool has_ignore,
     long ignore, int lanes) {
+  constexpr int VE = kWidth<T>;
   const int rows = 256 / lanes;
   const long t = blockIdx.x * (long)rows + threadIdx.x / lanes;
   if (t >= n) return;
   const long id = ids[t];
   const bool skip = has_ignore && id == ignore;
   const bool bad = id < 0 || id >= vocab;
-  const T* src = w + (skip || bad ? 0 : id * stride);
+  const T* src = w + id * stride;
   T* dst = y + t * dim;
-  const float none = skip ? 0.f : __builtin_nanf("");
   const long step = (long)lanes * VE;
-#pragma unroll 4
-  for (long c = (threadIdx.x % lanes) * VE; c < dim; c += step) {
+  if (skip || bad) {
     float r[VE];
-    if (skip || bad) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) r[i] = none;
-    } else {
-      load<T, VE>(src + c, r);
+    for (int i = 0; i < VE; ++i) r[i] = skip ? 0.f : __builtin_nanf("");
+    for (long c = (threadIdx.x % lanes) * VE; c < dim; c += step)
+      store<T, VE, true>(dst + column<VE>(c, dim), r, dim);
+    return;
+  }
+  constexpr int U = 4;  // vectors in flight
+  for (long c0 = (threadIdx.x % lanes) * VE; c0 < dim; c0 += U * step) {
+    float r[U][VE];
 #pragma unroll
-      for (int i = 0; i < VE; ++i) r[i] *= scale;
+    for (int u = 0; u < U; ++u)
+      load<T, VE>(src + column<VE>(c0 + u * step, dim), r[u], dim);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c0 + u * step >= dim) break;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) r[u][i] *= scale;
+      store<T, VE, true>(dst + column<VE>(c0 + u * step, dim), r[u], dim);
     }
-    store<T, VE>(dst + c, r);
   }
 }
 
@@ -77,119 +96,217 @@ __device__ __forceinline__ unsigned long long same_bin(
   return among;
 }
 
-// order[0..m): the tokens by id, those of one id in their own order;
-// sorted[0..m): their ids; offsets[v]: the first place of id v, offsets
-// [vocab] = m.  Tokens that are ignored or out of range are left out.
-template <typename I>
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
-    const I* __restrict__ ids, long n, long vocab, int range, int bits,
-    bool has_ignore, long ignore, int* __restrict__ order,
-    int* __restrict__ sorted, int* __restrict__ offsets) {
-  extern __shared__ int count[];  // [wave][range]
-  __shared__ int below[kSortWaves];
-  __shared__ int scan[kSortWaves];
+// The exclusive sum over a workgroup of WAVES waves, and the whole sum.
+template <int WAVES>
+__device__ __forceinline__ int scan(int v, int* lds, int* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long lo = blockIdx.x * (long)range;
-  const long hi = lo + range < vocab ? lo + range : vocab;
-  const long per = (n + kSortThreads - 1) / kSortThreads * 64;
-  const long begin = wave * per;
-  const long end = begin + per < n ? begin + per : n;
-  int* mine = count + wave * range;
-  for (int i = threadIdx.x; i < kSortWaves * range; i += kSortThreads)
-    count[i] = 0;
-  __syncthreads();
-
-  constexpr int U = 8;  // loads in flight
-  int less = 0;
-  for (long base = begin; base < end; base += 64 * U) {
-    long id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long t = base + u * 64 + lane;
-      id[u] = t < end ? id_at(ids, t, vocab, has_ignore, ignore) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      less += id[u] >= 0 && id[u] < lo;
-      const bool in = id[u] >= lo && id[u] < hi;
-      const unsigned long long any = __ballot(in);
-      if (any == 0) continue;
-      const int bin = in ? int(id[u] - lo) : 0;
-      const unsigned long long eq = same_bin(any, bin, bits);
-      if (in && lane == __ffsll(eq) - 1) atomicAdd(&mine[bin], __popcll(eq));
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) less += __shfl_xor(less, off, 64);
-  if (lane == 0) below[wave] = less;
-  __syncthreads();
-
-  // every bin's first place, and every wave's within the bin
-  int start = 0;
-  for (int i = 0; i < kSortWaves; ++i) start += below[i];
-  const int bin0 = threadIdx.x;
-  int total = 0;
-  if (bin0 < range)
-    for (int i = 0; i < kSortWaves; ++i) total += count[i * range + bin0];
-  int incl = total;
+  int incl = v;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int up = __shfl_up(incl, off, 64);
     if (lane >= off) incl += up;
   }
-  if (lane == 63) scan[wave] = incl;
+  if (lane == 63) lds[wave] = incl;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) start += scan[i];
-  start += incl - total;
-  if (bin0 < range) {
-    int at = start;
-    for (int i = 0; i < kSortWaves; ++i) {
-      const int c = count[i * range + bin0];
-      count[i * range + bin0] = at;
-      at += c;
+  int before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    if (i < wave) before += lds[i];
+    total += lds[i];
+  }
+  __syncthreads();
+  *all = total;
+  return before + incl - v;
+}
+
+// A stable counting sort of `n` items by a workgroup: fetch(p) is item p (an
+// id and a token, or a negative id), bin(item) its bin or -1 for none, and
+// emit(item, place) gets its place.  count is [WAVES][bins], and begin(bin,
+// first, n) gets each bin's first place and size.  Each wave takes a run of
+// the items, four of each lane's at once.
+template <int WAVES, typename F, typename B, typename G, typename E>
+__device__ __forceinline__ void counting_sort(long n, int bins, int bits,
+                                              int* count, int* lds, F fetch,
+                                              B bin, G begin, E emit) {
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long per = (n + 64 * WAVES - 1) / (64 * WAVES) * 64;
+  const long first = wave * per, last = first + per < n ? first + per : n;
+  int* mine = count + wave * bins;
+  for (int i = threadIdx.x; i < WAVES * bins; i += 64 * WAVES) count[i] = 0;
+  __syncthreads();
+  for (long p0 = first; p0 < last; p0 += 64 * U) {
+    int2 it[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long p = p0 + u * 64 + lane;
+      it[u] = p < last ? fetch(p) : make_int2(-1, 0);
     }
-    if (lo + bin0 < vocab) {
-      offsets[lo + bin0] = start;
-      if (lo + bin0 == vocab - 1) offsets[vocab] = at;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = it[u].x >= 0 ? bin(it[u]) : -1;
+      const unsigned long long any = __ballot(b >= 0);
+      if (any == 0) continue;
+      const unsigned long long eq = same_bin(any, b, bits);
+      if (b >= 0 && lane == __ffsll(eq) - 1)
+        atomicAdd(&mine[b], __popcll(eq));
     }
   }
   __syncthreads();
-
-  for (long base = begin; base < end; base += 64 * U) {
-    long id[U];
+  int before = 0;  // of the bins of earlier rounds
+  for (int b0 = 0; b0 < bins; b0 += 64 * WAVES) {
+    const int b = b0 + threadIdx.x;
+    int total = 0, all;
+    if (b < bins)
+      for (int i = 0; i < WAVES; ++i) total += count[i * bins + b];
+    int at = before + scan<WAVES>(total, lds, &all);
+    before += all;
+    if (b < bins) {
+      begin(b, at, total);
+      for (int i = 0; i < WAVES; ++i) {
+        const int c = count[i * bins + b];
+        count[i * bins + b] = at;
+        at += c;
+      }
+    }
+  }
+  __syncthreads();
+  for (long p0 = first; p0 < last; p0 += 64 * U) {
+    int2 it[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long t = base + u * 64 + lane;
-      id[u] = t < end ? id_at(ids, t, vocab, has_ignore, ignore) : -1;
+      const long p = p0 + u * 64 + lane;
+      it[u] = p < last ? fetch(p) : make_int2(-1, 0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool in = id[u] >= lo && id[u] < hi;
-      const unsigned long long any = __ballot(in);
+      const int b = it[u].x >= 0 ? bin(it[u]) : -1;
+      const unsigned long long any = __ballot(b >= 0);
       if (any == 0) continue;
-      const int bin = in ? int(id[u] - lo) : 0;
-      const unsigned long long eq = same_bin(any, bin, bits);
-      const int leader = in ? __ffsll(eq) - 1 : lane;
-      int first = 0;
-      if (in && lane == leader) first = atomicAdd(&mine[bin], __popcll(eq));
-      first = __shfl(first, leader, 64);
-      if (in) {
-        const int at = first + __popcll(eq & ((1ull << lane) - 1));
-        order[at] = int(base + u * 64 + lane);
-        sorted[at] = int(id[u]);
-      }
+      const unsigned long long eq = same_bin(any, b, bits);
+      const int leader = b >= 0 ? __ffsll(eq) - 1 : lane;
+      int at = 0;
+      if (b >= 0 && lane == leader) at = atomicAdd(&mine[b], __popcll(eq));
+      at = __shfl(at, leader, 64) + __popcll(eq & ((1ull << lane) - 1));
+      if (b >= 0) emit(it[u], at);
     }
   }
 }
 
-// Waves 0 .. chunks * slices - 1: the sums of 32 sorted tokens over a slice
-// of 64 * VE columns.  The waves behind them zero the rows without a token.
-template <typename T, int VE>
+// A piece of the tokens, sorted by bucket: piece[0..) are (id, token), and
+// starts[bucket][workgroup] each bucket's first place, up to one behind the
+// last bucket.  Tokens that are ignored or out of range are left out.
+template <typename I>
+__global__ __launch_bounds__(kSplitThreads) void embed_split_kernel(
+    const I* __restrict__ ids, long n, long vocab, long per, int bucket_bits,
+    bool has_ignore, long ignore, int2* __restrict__ pieces,
+    int* __restrict__ starts) {
+  extern __shared__ int count[];  // [wave][buckets]
+  __shared__ int lds[kSplitWaves];
+  const long p0 = blockIdx.x * per;
+  const long here = p0 + per < n ? per : n - p0;
+  const int buckets = 1 << bucket_bits;
+  counting_sort<kSplitWaves>(
+      here, buckets, bucket_bits, count, lds,
+      [&](long p) {
+        return make_int2(
+            int(id_at(ids, p0 + p, vocab, has_ignore, ignore)), int(p0 + p));
+      },
+      [&](int2 it) { return it.x & (buckets - 1); },
+      [&](int b, int at, int size) {
+        starts[(long)b * gridDim.x + blockIdx.x] = at;
+        if (b == buckets - 1)
+          starts[(long)buckets * gridDim.x + blockIdx.x] = at + size;
+      },
+      [&](int2 it, int at) { pieces[p0 + at] = it; });
+}
+
+// A bucket of all pieces, or `bins` of its ids, sorted by id.  order[0..m):
+// the tokens, those of one id in their own order; sorted[0..m): their ids;
+// range[v]: the places of id v; *tokens = m.
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
+    const int2* __restrict__ pieces, const int* __restrict__ starts, int n,
+    long per, long vocab, int bucket_bits, int bins, int bits, int parts,
+    int* __restrict__ order, int* __restrict__ sorted,
+    int2* __restrict__ range, int* __restrict__ tokens) {
+  extern __shared__ int count[];  // [wave][bins]
+  __shared__ int piece[kMaxPieces + 1];  // first item of a piece in the list
+  __shared__ int from[kMaxPieces];       // and its place in the pieces
+  __shared__ int lds[kSortWaves];
+  __shared__ int below;
+  const int bucket = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int* a = starts + (long)bucket * n;
+  int items = 0, place = 0, all;
+  for (int g0 = 0; g0 < n; g0 += kSortThreads) {
+    const int g = g0 + threadIdx.x;
+    const int at = g < n ? a[g] : 0, size = g < n ? a[n + g] - at : 0;
+    const int first = scan<kSortWaves>(size, lds, &all);
+    if (g < n) {
+      piece[g] = items + first;
+      from[g] = int(g * per) + at;
+    }
+    items += all;
+    scan<kSortWaves>(at, lds, &all);
+    place += all;
+  }
+  if (threadIdx.x == 0) {
+    piece[n] = items;
+    below = 0;
+  }
+  if (blockIdx.x == 0) {
+    int m = 0;
+    for (int g = threadIdx.x; g < n; g += kSortThreads)
+      m += starts[((long)n << bucket_bits) + g];
+    scan<kSortWaves>(m, lds, &all);
+    if (threadIdx.x == 0) *tokens = all;
+  }
+  __syncthreads();
+  auto item = [&](long p) {
+    int lo = 0, hi = n - 1;  // the last piece that begins at or before p
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (piece[mid] <= p) lo = mid;
+      else hi = mid - 1;
+    }
+    return pieces[from[lo] + (int(p) - piece[lo])];
+  };
+  const int bin0 = part * bins;
+  if (part > 0) {  // what the bucket's parts before this one hold
+    int less = 0;
+    for (int p = threadIdx.x; p < items; p += kSortThreads)
+      less += (item(p).x >> bucket_bits) < bin0;
+    atomicAdd(&below, less);
+    __syncthreads();
+    place += below;
+  }
+  counting_sort<kSortWaves>(
+      items, bins, bits, count, lds, item,
+      [&](int2 it) {
+        const int b = (it.x >> bucket_bits) - bin0;
+        return b >= 0 && b < bins ? b : -1;
+      },
+      [&](int b, int at, int size) {
+        const long id = ((long)(bin0 + b) << bucket_bits) + bucket;
+        if (id < vocab)
+          range[id] = make_int2(place + at, place + at + size);
+      },
+      [&](int2 it, int at) {
+        order[place + at] = it.y;
+        sorted[place + at] = it.x;
+      });
+}
+
+// Waves 0 .. chunks * slices - 1: the sums of `size` sorted tokens over a
+// slice of 64 * VE columns.  The waves behind them zero the rows without a
+// token.
+template <typename T>
 __global__ __launch_bounds__(256) void embed_rows_kernel(
     const T* __restrict__ gy, const int* __restrict__ order,
-    const int* __restrict__ sorted, const int* __restrict__ offsets,
-    T* __restrict__ dw, float* __restrict__ head, float* __restrict__ tail,
-    long vocab, long dim, int chunks, int slices, float scale) {
+    const int* __restrict__ sorted, const int2* __restrict__ range,
+    const int* __restrict__ tokens, T* __restrict__ dw,
+    float* __restrict__ head, float* __restrict__ tail,
+    long vocab, long dim, int size, int chunks, int slices, float scale) {
+  constexpr int VE = kWidth<T>;
   const int lane = threadIdx.x & 63;
   long wave = blockIdx.x * 4l + (threadIdx.x >> 6);
   const long sums = (long)chunks * slices;
@@ -199,19 +316,21 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(
 #pragma unroll
     for (int i = 0; i < VE; ++i) z[i] = 0.f;
     for (long v = wave - sums; v < vocab; v += waves) {
-      if (offsets[v] != offsets[v + 1]) continue;
+      const int2 r = range[v];
+      if (r.x != r.y) continue;
       for (long c = lane * VE; c < dim; c += 64 * VE)
-        store<T, VE>(dw + v * dim + c, z);
+        store<T, VE, true>(dw + v * dim + column<VE>(c, dim), z, dim);
     }
     return;
   }
   const int chunk = __builtin_amdgcn_readfirstlane(int(wave / slices));
-  const long col = (wave % slices) * 64 * VE + lane * VE;
-  const int m = offsets[vocab];
-  const int p0 = chunk * kChunk;
-  if (p0 >= m) return;
-  const int len = m - p0 < kChunk ? m - p0 : kChunk;
+  long col = (wave % slices) * 64 * VE + lane * VE;
   const bool on = col < dim;
+  col = column<VE>(col, dim);
+  const int m = *tokens;
+  const int p0 = chunk * size;
+  if (p0 >= m) return;
+  const int len = m - p0 < size ? m - p0 : size;
   const int at = p0 + (lane < len ? lane : 0);
   const int my_tok = order[at], my_id = sorted[at];
   // whether the row goes on in the neighbouring chunks
@@ -227,12 +346,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int tok = __shfl(my_tok, j0 + u < len ? j0 + u : 0, 64);
-      if (on && j0 + u < len) {
-        load<T, VE>(gy + tok * dim + col, g[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) g[u][i] = 0.f;
-      }
+      load<T, VE>(gy + tok * dim + col, g[u], dim);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -246,13 +360,13 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(
       if (j + 1 < len && next == id) continue;
       // the row ends here, or the chunk does
       if (first && before) {
-        if (on) store<float, VE>(head + chunk * dim + col, acc);
+        if (on) store<float, VE>(head + chunk * dim + col, acc, dim);
       } else if (j + 1 == len && after) {
-        if (on) store<float, VE>(tail + chunk * dim + col, acc);
+        if (on) store<float, VE>(tail + chunk * dim + col, acc, dim);
       } else if (on) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) acc[i] *= scale;
-        store<T, VE>(dw + id * dim + col, acc);
+        store<T, VE, true>(dw + id * dim + col, acc, dim);
       }
       first = false;
 #pragma unroll
@@ -261,46 +375,78 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(
   }
 }
 
-// A workgroup of a chunk in which a row begins that goes on behind it: its
-// tail there and the heads of the chunks up to the row's last token.
-template <typename T, int VE>
+// A row that begins in a chunk and goes on behind it: its tail there and the
+// heads of the chunks up to its last token.  A wave has a chunk; rows of more
+// than 16 parts are then summed by all eight waves.
+template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(
-    const int* __restrict__ sorted, const int* __restrict__ offsets,
-    const float* __restrict__ head, const float* __restrict__ tail,
-    T* __restrict__ dw, long vocab, long dim, float scale) {
+    const int* __restrict__ sorted, const int2* __restrict__ range,
+    const int* __restrict__ tokens, const float* __restrict__ head,
+    const float* __restrict__ tail, T* __restrict__ dw, long dim, int size,
+    float scale) {
+  constexpr int VE = kWidth<T>;
   __shared__ float part[kJoinWaves][64 * VE];
-  const int chunk = blockIdx.x;
-  const int m = offsets[vocab];
-  const int p1 = (chunk + 1) * kChunk;
-  if (p1 >= m) return;
-  const int id = sorted[p1];
-  if (sorted[p1 - 1] != id || offsets[id] < chunk * kChunk) return;
-  const int last = (offsets[id + 1] - 1) / kChunk;
+  __shared__ int3 rows[kJoinWaves];  // of many parts: id, first, last chunk
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long col = blockIdx.y * 64l * VE + lane * VE;
-  float acc[VE];
+  long col = blockIdx.y * 64l * VE + lane * VE;
+  const bool on = col < dim;
+  col = column<VE>(col, dim);
+  const int m = *tokens;
+
+  // the parts of a row that are `step` chunks apart
+  auto sum = [&](int chunk, int from, int last, int step, float (&acc)[VE]) {
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
-  if (col < dim) {
-    if (wave == 0) load<float, VE>(tail + chunk * dim + col, acc);
+    for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+    if (!on) return;
+    if (from == chunk + 1)
+      load<float, VE>(tail + chunk * dim + col, acc, dim);
 #pragma unroll 8
-    for (int c = chunk + 1 + wave; c <= last; c += kJoinWaves) {
+    for (int c = from; c <= last; c += step) {
       float r[VE];
-      load<float, VE>(head + c * dim + col, r);
+      load<float, VE>(head + c * dim + col, r, dim);
 #pragma unroll
       for (int i = 0; i < VE; ++i) acc[i] += r[i];
     }
+  };
+  auto finish = [&](int id, float (&acc)[VE]) {
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] *= scale;
+    store<T, VE, true>(dw + id * dim + col, acc, dim);
+  };
+
+  const int chunk = blockIdx.x * kJoinWaves + wave;
+  const long p1 = (chunk + 1l) * size;
+  int3 row = make_int3(-1, 0, 0);
+  if (p1 < m && sorted[p1 - 1] == sorted[p1]) {
+    const int id = sorted[p1];
+    const int2 r = range[id];
+    if (r.x >= p1 - size) row = make_int3(id, chunk, (r.y - 1) / size);
   }
-#pragma unroll
-  for (int i = 0; i < VE; ++i) part[wave][lane * VE + i] = acc[i];
+  const bool many = row.z - row.y > 16;
+  if (lane == 0) rows[wave] = many ? row : make_int3(-1, 0, 0);
+  if (row.x >= 0 && !many) {
+    float acc[VE];
+    sum(row.y, row.y + 1, row.z, 1, acc);
+    finish(row.x, acc);
+  }
   __syncthreads();
-  if (wave != 0 || col >= dim) return;
-  for (int w = 1; w < kJoinWaves; ++w)
+  for (int k = 0; k < kJoinWaves; ++k) {
+    const int3 r = rows[k];
+    if (r.x < 0) continue;  // for all waves alike
+    float acc[VE];
+    sum(r.y, r.y + 1 + wave, r.z, kJoinWaves, acc);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] += part[w][lane * VE + i];
+    for (int i = 0; i < VE; ++i) part[wave][lane * VE + i] = acc[i];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] *= scale;
-  store<T, VE>(dw + id * dim + col, acc);
+        for (int i = 0; i < VE; ++i) acc[i] += part[w][lane * VE + i];
+      finish(r.x, acc);
+    }
+    __syncthreads();
+  }
 }
 
 void check_ids(const torch::Tensor& ids, const char* what) {
@@ -326,18 +472,17 @@ torch::Tensor embed_lookup(torch::Tensor ids, torch::Tensor w, double scale,
   shape.push_back(dim);
   auto y = torch::empty(shape, w.options());
   if (n == 0) return y;
-  int ve = vector_width(w.data_ptr(), dim, w.stride(0), w.element_size());
-  const long nvec = dim / ve;
+  const int ve = 16 / (int)w.element_size();
+  const long nvec = (dim + ve - 1) / ve;
   int lanes = 64;  // of a row; a wave takes several short ones
   while (lanes > 1 && lanes / 2 >= nvec) lanes /= 2;
   const long blocks = (n + 256 / lanes - 1) / (256 / lanes);
   TORCH_CHECK(blocks < (1l << 31), "embed_lookup: too many tokens");
-  dispatch_vec(w.scalar_type(), ve, "embed_lookup", [&](auto t, auto width) {
+  dispatch(w.scalar_type(), "embed_lookup", [&](auto t) {
     using T = decltype(t);
-    constexpr int VE = decltype(width)::value;
     auto go = [&](auto i) {
       using I = decltype(i);
-      embed_lookup_kernel<T, VE, I><<<dim3(blocks), dim3(256), 0, stream()>>>(
+      embed_lookup_kernel<T, I><<<dim3(blocks), dim3(256), 0, stream()>>>(
           (const I*)ids.data_ptr(), (const T*)w.data_ptr(),
           (T*)y.data_ptr(), n, w.size(0), dim, w.stride(0), (float)scale,
           has_ignore, ignore, lanes);
@@ -358,56 +503,83 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
               gy.numel() == n * gy.size(-1) && vocab > 0,
               "embed_grad: gy must be contiguous, one row for each id");
   // places and ids are held in 32 bits
-  TORCH_CHECK(n < (1l << 31) - 64 * kSortThreads && vocab < (1l << 31) - 1,
-              "embed_grad: fewer than 2^31 tokens and rows");
+  TORCH_CHECK(n < (1l << 30) && vocab < (1l << 30),
+              "embed_grad: fewer than 2^30 tokens and rows");
   const c10::DeviceGuard guard(gy.device());
   const long dim = gy.size(-1);
   auto dw = torch::empty({vocab, dim}, gy.options());
-  const auto ints = gy.options().dtype(at::kInt);
-  // a range for each of 256 workgroups, or as many as 1024 ids each take
-  int range = int((vocab + 255) / 256);
-  if (range > kMaxBins) range = kMaxBins;
+  // 256 buckets, or as many as leave 1024 ids to each; above 2^19 ids a
+  // bucket is sorted in parts
+  int bucket_bits = 0;
+  while (bucket_bits < 8 && (1l << bucket_bits) < vocab) ++bucket_bits;
+  while (bucket_bits < 9 && (vocab >> bucket_bits) >= kMaxBins) ++bucket_bits;
+  const int buckets = 1 << bucket_bits;
+  const long of_bucket = (vocab + buckets - 1) / buckets;
+  const int bins = int(of_bucket < kMaxBins ? of_bucket : kMaxBins);
+  const int parts = int((of_bucket + bins - 1) / bins);
   int bits = 0;
-  while ((1 << bits) < range) ++bits;
-  const int groups = int((vocab + range - 1) / range);
-  auto places = torch::empty({2 * n + vocab + 1}, ints);
-  int* order = places.data_ptr<int>();
+  while ((1 << bits) < bins) ++bits;
+  // pieces of 1024 tokens, or as many as make 1024 pieces
+  const long per = std::max((long)kSplitThreads,
+                            (n + kMaxPieces * 64l - 1) / (kMaxPieces * 64l) *
+                                64);
+  const int pieces = int((n + per - 1) / per);
+  const long starts = (buckets + 1l) * pieces;
+  auto space = torch::empty({4 * n + 2 * vocab + starts + 1},
+                            gy.options().dtype(at::kInt));
+  int2* range = reinterpret_cast<int2*>(space.data_ptr<int>());
+  int2* piece = range + vocab;
+  int* order = reinterpret_cast<int*>(piece + n);
   int* sorted = order + n;
-  int* offsets = sorted + n;
-  const int lds = kSortWaves * range * (int)sizeof(int);
-  auto sort = [&](auto i) {
-    using I = decltype(i);
-    embed_sort_kernel<I><<<dim3(groups), dim3(kSortThreads), lds, stream()>>>(
-        (const I*)ids.data_ptr(), n, vocab, range, bits, has_ignore, ignore,
-        order, sorted, offsets);
-  };
-  if (ids.scalar_type() == at::kLong) sort(long());
-  else sort(int());
+  int* start = sorted + n;
+  int* tokens = start + starts;
+  if (n) {
+    const int lds = kSplitWaves * buckets * (int)sizeof(int);
+    auto split = [&](auto i) {
+      using I = decltype(i);
+      embed_split_kernel<I>
+          <<<dim3(pieces), dim3(kSplitThreads), lds, stream()>>>(
+              (const I*)ids.data_ptr(), n, vocab, per, bucket_bits,
+              has_ignore, ignore, piece, start);
+    };
+    if (ids.scalar_type() == at::kLong) split(long());
+    else split(int());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  }
+  embed_sort_kernel<<<dim3(buckets * parts), dim3(kSortThreads),
+                      kSortWaves * bins * (int)sizeof(int), stream()>>>(
+      piece, start, pieces, per, vocab, bucket_bits, bins, bits, parts,
+      order, sorted, range, tokens);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 
-  const int ve = vector_width(gy.data_ptr(), dim, dim, gy.element_size());
-  const int chunks = int((n + kChunk - 1) / kChunk);
-  auto parts = torch::empty({2, chunks, dim},
-                            gy.options().dtype(at::kFloat));
-  float* head = parts.data_ptr<float>();
-  float* tail = head + (long)chunks * dim;
+  const int ve = 16 / (int)gy.element_size();
   const int slices = int((dim + 64 * ve - 1) / (64 * ve));
+  // sorted tokens of a wave: 32, or fewer until four waves have work on each
+  // SIMD (22500 rows of 1520 bytes at 16: 32 us, at 32: 35 us)
+  int size = 32;
+  while (size > 8 && (n + size - 1) / size * slices < 4096) size /= 2;
+  const int chunks = int((n + size - 1) / size);
+  auto sums = torch::empty({2, chunks, dim},
+                            gy.options().dtype(at::kFloat));
+  float* head = sums.data_ptr<float>();
+  float* tail = head + (long)chunks * dim;
   const long zero_waves = vocab < 4096 ? vocab : 4096;
   const long blocks = ((long)chunks * slices + zero_waves + 3) / 4;
   TORCH_CHECK(blocks < (1l << 31) && slices < 65536,
               "embed_grad: too many elements");
-  dispatch_vec(gy.scalar_type(), ve, "embed_grad", [&](auto t, auto width) {
+  dispatch(gy.scalar_type(), "embed_grad", [&](auto t) {
     using T = decltype(t);
-    constexpr int VE = decltype(width)::value;
-    embed_rows_kernel<T, VE><<<dim3(blocks), dim3(256), 0, stream()>>>(
-        (const T*)gy.data_ptr(), order, sorted, offsets, (T*)dw.data_ptr(),
-        head, tail, vocab, dim, chunks, slices, (float)scale);
+    embed_rows_kernel<T><<<dim3(blocks), dim3(256), 0, stream()>>>(
+        (const T*)gy.data_ptr(), order, sorted, range, tokens,
+        (T*)dw.data_ptr(), head, tail, vocab, dim, size, chunks, slices,
+        (float)scale);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     if (chunks > 1)
-      embed_join_kernel<T, VE>
-          <<<dim3(chunks, slices), dim3(64 * kJoinWaves), 0, stream()>>>(
-              sorted, offsets, head, tail, (T*)dw.data_ptr(), vocab, dim,
-              (float)scale);
+      embed_join_kernel<T>
+          <<<dim3((chunks + kJoinWaves - 1) / kJoinWaves, slices),
+             dim3(64 * kJoinWaves), 0, stream()>>>(
+              sorted, range, tokens, head, tail, (T*)dw.data_ptr(), dim,
+              size, (float)scale);
   });
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return dw;

@@ -1018,7 +1018,7 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
   v = rows_of(v);
   auto o = torch::empty({b, h, dv}, q.options());
   if (b * h == 0) return o;
-  const int ve = vector_width(state.data_ptr(), dv, dv, 4);
+  const bool wide = dv % 4 == 0;
   dispatch(q.scalar_type(), "linear_attention_step", [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto width) {
@@ -1032,7 +1032,7 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
                          k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                          (float)scale);
     };
-    if (ve == 4) go(std::integral_constant<int, 4>());
+    if (wide) go(std::integral_constant<int, 4>());
     else go(std::integral_constant<int, 1>());
   });
   C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -8,11 +8,11 @@
 //   dh = rstd * (g - xhat * mean(g * xhat)) + gh,   dw = sum_rows gy * xhat.
 //
 // A row stays in registers: every input is read once and every output
-// written once, which bounds all three kernels.  y is computed from the
-// unrounded sum; the backward pass reads the rounded one, so its xhat is
-// off by half a step of the type.  Sums and rstd are fp32.
+// written once, which bounds all three kernels.  The sum is fp32 wherever it
+// is used; the backward pass adds x and the residual again, since the rounded
+// sum would leave its rounding in dw.  Sums and rstd are fp32.
 //
-// A row belongs to `tpr` threads: a wave where it fits, or a workgroup.
+// A row belongs to `tpr` threads, a wave or several, of 16 elements each.
 
 #include "seq_common.h"
 
@@ -22,9 +22,11 @@ using namespace seq;
 
 constexpr int kMaxDim = 16384;
 
-// vectors of a row that a thread holds: 16 to 32 elements
-template <int VE>
-constexpr int kHeld = VE >= 4 ? 4 : VE == 2 ? 8 : 16;
+// vectors of a row that a thread holds
+template <typename T>
+constexpr int kHeld = 16 / kWidth<T>;
+template <typename T>
+using Part = float[kHeld<T>][kWidth<T>];
 
 // The sum over the row's threads, for all of them.  `lds` holds one float
 // for each wave of the workgroup and is written again by the next call, so
@@ -54,70 +56,94 @@ __device__ __forceinline__ float row_max(float v, int tpr, float* lds) {
   return v;
 }
 
-template <typename T, int VE>
-__device__ __forceinline__ void load_weight(const void* w, bool w32, long c,
-                                            float (&r)[VE]) {
-  if (w32) load<float, VE>((const float*)w + c, r);
-  else load<T, VE>((const T*)w + c, r);
+// A thread's part of the weight.
+template <typename T>
+__device__ __forceinline__ void load_weight(const void* w, bool w32, int dim,
+                                            int t, int tpr,
+                                            Part<T>& r) {
+  constexpr int VE = kWidth<T>;
+#pragma unroll
+  for (int k = 0; k < kHeld<T>; ++k) {
+    const int c = (k * tpr + t) * VE;
+    if (c >= dim) continue;
+    if (w32) load<float, VE>((const float*)w + c, r[k], dim - c);
+    else load<T, VE>((const T*)w + c, r[k], dim - c);
+  }
+}
+
+// A thread's part of a row, zero behind its end.
+template <typename T>
+__device__ __forceinline__ void load_row(const T* x, int dim, int t, int tpr,
+                                         Part<T>& r) {
+  constexpr int VE = kWidth<T>;
+#pragma unroll
+  for (int k = 0; k < kHeld<T>; ++k) {
+    const int c = (k * tpr + t) * VE;
+    if (c < dim) {
+      load<T, VE>(x + c, r[k], dim - c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) r[k][i] = 0.f;
+    }
+  }
 }
 
 // h of a row and its rstd; the sum is written to `sum` if there is one.
-template <typename T, int VE>
+template <typename T>
 __device__ __forceinline__ float read_row(
     const T* x, const T* res, T* sum, int dim, int t, int tpr, float eps,
-    float* lds, float (&h)[kHeld<VE>][VE]) {
+    float* lds, Part<T>& h) {
+  constexpr int VE = kWidth<T>;
+  load_row<T>(x, dim, t, tpr, h);
+  if (res) {
+    Part<T> r;
+    load_row<T>(res, dim, t, tpr, r);
+#pragma unroll
+    for (int k = 0; k < kHeld<T>; ++k) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) h[k][i] += r[k][i];
+      const int c = (k * tpr + t) * VE;
+      if (c < dim) store<T, VE, true>(sum + c, h[k], dim - c);
+    }
+  }
   float sq = 0.f;
 #pragma unroll
-  for (int k = 0; k < kHeld<VE>; ++k) {
-    const int c = (k * tpr + t) * VE;
-    if (c < dim) {
-      load<T, VE>(x + c, h[k]);
-      if (res) {
-        float r[VE];
-        load<T, VE>(res + c, r);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) h[k][i] += r[i];
-        store<T, VE>(sum + c, h[k]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) h[k][i] = 0.f;
-    }
+  for (int k = 0; k < kHeld<T>; ++k)
 #pragma unroll
     for (int i = 0; i < VE; ++i) sq += h[k][i] * h[k][i];
-  }
   return rsqrtf(row_sum(sq, tpr, lds) / dim + eps);
 }
 
-template <typename T, int VE>
+template <typename T>
 __global__ __launch_bounds__(1024) void rms_fwd_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
     const void* __restrict__ w, bool w32, T* __restrict__ y,
     T* __restrict__ sum, float* __restrict__ rstd_out, long rows, int dim,
     long xs, long rs, int tpr, float eps) {
+  constexpr int VE = kWidth<T>;
   __shared__ float lds[2][16];
   const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
+  Part<T> wt;
+  load_weight<T>(w, w32, dim, t, tpr, wt);
   int turn = 0;
   for (long r0 = blockIdx.x * (long)per; r0 < rows;
        r0 += gridDim.x * (long)per, turn ^= 1) {
     long row = r0 + threadIdx.x / tpr;
     const bool on = row < rows;  // whole waves, and all of them at barriers
     if (!on) row = rows - 1;
-    float h[kHeld<VE>][VE];
-    const float rstd = read_row<T, VE>(
+    Part<T> h;
+    const float rstd = read_row<T>(
         x + row * xs, res ? res + row * rs : nullptr, sum + row * dim, dim, t,
         tpr, eps, lds[turn], h);
     if (!on) continue;
     if (rstd_out && t == 0) rstd_out[row] = rstd;
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
+    for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
       if (c < dim) {
-        float wt[VE];
-        load_weight<T, VE>(w, w32, c, wt);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) h[k][i] = h[k][i] * rstd * wt[i];
-        store<T, VE>(y + row * dim + c, h[k]);
+        for (int i = 0; i < VE; ++i) h[k][i] = h[k][i] * rstd * wt[k][i];
+        store<T, VE, true>(y + row * dim + c, h[k], dim - c);
       }
     }
   }
@@ -128,69 +154,70 @@ __device__ __forceinline__ float e4m3_scale(float amax) {
   return s > 0.f ? s : 1.f;  // a row of zeros
 }
 
-template <int VE>
+// Four values as e4m3 bytes, rounded to nearest even.
+__device__ __forceinline__ unsigned to_e4m3(float a, float b, float c,
+                                            float d) {
+  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true);
+}
+
+template <int N>
 __device__ __forceinline__ void store_e4m3(unsigned char* p, float scale,
-                                           const float (&y)[VE]) {
-  float q[VE];
+                                           const float (&y)[N], int n) {
+  float q[N];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
+  for (int i = 0; i < N; ++i) {
     const float v = y[i] / scale;
     // comparisons keep NaN
     q[i] = v > 448.f ? 448.f : v < -448.f ? -448.f : v;
   }
-  if constexpr (VE >= 4) {
-    unsigned u[VE / 4];
+  vec<unsigned, N / 4> u;
 #pragma unroll
-    for (int i = 0; i < VE / 4; ++i) {
-      int b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0,
-                                              false);
-      b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], b,
-                                          true);
-      u[i] = b;
-    }
-    if constexpr (VE == 8)
-      *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-    else
-      *reinterpret_cast<unsigned*>(p) = u[0];
+  for (int i = 0; i < N / 4; ++i)
+    u[i] = to_e4m3(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+  if (n >= N) {
+    typedef vec<unsigned, N / 4> bytes __attribute__((aligned(1)));
+    *reinterpret_cast<bytes*>(p) = u;
   } else {
 #pragma unroll
-    for (int i = 0; i < VE; ++i)
-      p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[i], q[i], 0, false) & 0xff;
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (u[i / 4] >> (i % 4 * 8)) & 0xff;
   }
 }
 
 // y in e4m3 with a scale for each row (group = 0) or each `group` columns,
 // 2^n of them that at most a wave holds: amax / 448.
-template <typename T, int VE>
+template <typename T>
 __global__ __launch_bounds__(1024) void rms_fp8_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
     const void* __restrict__ w, bool w32, unsigned char* __restrict__ q,
     float* __restrict__ scales, T* __restrict__ sum, long rows, int dim,
     long xs, long rs, int tpr, float eps, int group) {
+  constexpr int VE = kWidth<T>;
   __shared__ float lds[2][16];
   __shared__ float top[2][16];
   const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
+  Part<T> wt;
+  load_weight<T>(w, w32, dim, t, tpr, wt);
   int turn = 0;
   for (long r0 = blockIdx.x * (long)per; r0 < rows;
        r0 += gridDim.x * (long)per, turn ^= 1) {
     long row = r0 + threadIdx.x / tpr;
     const bool on = row < rows;
     if (!on) row = rows - 1;
-    float h[kHeld<VE>][VE];
-    const float rstd = read_row<T, VE>(
+    Part<T> h;
+    const float rstd = read_row<T>(
         x + row * xs, res ? res + row * rs : nullptr, sum + row * dim, dim, t,
         tpr, eps, lds[turn], h);
     float amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
+    for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
       float m = 0.f;
       if (c < dim) {
-        float wt[VE];
-        load_weight<T, VE>(w, w32, c, wt);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          h[k][i] = h[k][i] * rstd * wt[i];
+          h[k][i] = h[k][i] * rstd * wt[k][i];
           m = fmaxf(m, fabsf(h[k][i]));
         }
       }
@@ -200,7 +227,7 @@ __global__ __launch_bounds__(1024) void rms_fp8_kernel(
         if (c < dim && on) {
           const float s = e4m3_scale(m);
           if (c % group == 0) scales[row * (dim / group) + c / group] = s;
-          store_e4m3<VE>(q + row * dim + c, s, h[k]);
+          store_e4m3<VE>(q + row * dim + c, s, h[k], dim - c);
         }
       }
       amax = fmaxf(amax, m);
@@ -210,27 +237,30 @@ __global__ __launch_bounds__(1024) void rms_fp8_kernel(
     if (!on) continue;
     if (t == 0) scales[row] = s;
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
+    for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
-      if (c < dim) store_e4m3<VE>(q + row * dim + c, s, h[k]);
+      if (c < dim) store_e4m3<VE>(q + row * dim + c, s, h[k], dim - c);
     }
   }
 }
 
 // dh of all rows, and the sum of gy * xhat over the workgroup's rows in
 // part[workgroup]: a thread's columns are the same for each of its rows.
-template <typename T, int VE>
+template <typename T>
 __global__ __launch_bounds__(1024) void rms_bwd_kernel(
-    const T* __restrict__ gy, const T* __restrict__ h,
-    const T* __restrict__ gh, const void* __restrict__ w, bool w32,
-    const float* __restrict__ rstd_in, T* __restrict__ dh,
-    float* __restrict__ part, long rows, int dim, long hs, int tpr) {
-  extern __shared__ float cols[];  // [dim], where a wave has a row
+    const T* __restrict__ gy, const T* __restrict__ x,
+    const T* __restrict__ res, const T* __restrict__ gh,
+    const void* __restrict__ w, bool w32, const float* __restrict__ rstd_in,
+    T* __restrict__ dh, float* __restrict__ part, long rows, int dim, long xs,
+    long rs, int tpr) {
+  extern __shared__ float cols[];  // [dim], where a workgroup has more rows
+  constexpr int VE = kWidth<T>;
   __shared__ float lds[2][16];
   const int t = threadIdx.x % tpr, per = blockDim.x / tpr;
-  float dw[kHeld<VE>][VE];
+  Part<T> wt, dw;
+  load_weight<T>(w, w32, dim, t, tpr, wt);
 #pragma unroll
-  for (int k = 0; k < kHeld<VE>; ++k)
+  for (int k = 0; k < kHeld<T>; ++k)
 #pragma unroll
     for (int i = 0; i < VE; ++i) dw[k][i] = 0.f;
   int turn = 0;
@@ -239,68 +269,74 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(
     long row = r0 + threadIdx.x / tpr;
     const bool on = row < rows;
     if (!on) row = rows - 1;
+    Part<T> g, xh, add;
+    load_row<T>(gy + row * dim, dim, t, tpr, g);
+    load_row<T>(x + row * xs, dim, t, tpr, xh);
+    if (res) {
+      Part<T> r;
+      load_row<T>(res + row * rs, dim, t, tpr, r);
+#pragma unroll
+      for (int k = 0; k < kHeld<T>; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) xh[k][i] += r[k][i];
+    }
+    if (gh) {
+      load_row<T>(gh + row * dim, dim, t, tpr, add);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kHeld<T>; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) add[k][i] = 0.f;
+    }
     const float rstd = rstd_in[row];
-    float g[kHeld<VE>][VE], xh[kHeld<VE>][VE];
     float dot = 0.f;
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
-      const int c = (k * tpr + t) * VE;
-      if (c < dim && on) {
-        float wt[VE];
-        load<T, VE>(gy + row * dim + c, g[k]);
-        load<T, VE>(h + row * hs + c, xh[k]);
-        load_weight<T, VE>(w, w32, c, wt);
+    for (int k = 0; k < kHeld<T>; ++k) {
+      if ((k * tpr + t) * VE >= dim || !on) continue;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          xh[k][i] *= rstd;
-          dw[k][i] += g[k][i] * xh[k][i];
-          g[k][i] *= wt[i];
-          dot += g[k][i] * xh[k][i];
-        }
+      for (int i = 0; i < VE; ++i) {
+        xh[k][i] *= rstd;
+        dw[k][i] += g[k][i] * xh[k][i];
+        g[k][i] *= wt[k][i];
+        dot += g[k][i] * xh[k][i];
       }
     }
     const float mean = row_sum(dot, tpr, lds[turn]) / dim;
     if (!on) continue;
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
+    for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
       if (c < dim) {
-        float add[VE];
-        if (gh) {
-          load<T, VE>(gh + row * dim + c, add);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) add[i] = 0.f;
-        }
 #pragma unroll
         for (int i = 0; i < VE; ++i)
-          add[i] += rstd * (g[k][i] - xh[k][i] * mean);
-        store<T, VE>(dh + row * dim + c, add);
+          add[k][i] += rstd * (g[k][i] - xh[k][i] * mean);
+        store<T, VE, true>(dh + row * dim + c, add[k], dim - c);
       }
     }
   }
   float* out = part + blockIdx.x * (long)dim;
   if (per == 1) {
 #pragma unroll
-    for (int k = 0; k < kHeld<VE>; ++k) {
+    for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
-      if (c < dim) store<float, VE>(out + c, dw[k]);
+      if (c < dim) store<float, VE>(out + c, dw[k], dim - c);
     }
     return;
   }
   for (int p = 0; p < per; ++p) {  // one row of threads after another
     if (threadIdx.x / tpr == p) {
 #pragma unroll
-      for (int k = 0; k < kHeld<VE>; ++k) {
+      for (int k = 0; k < kHeld<T>; ++k) {
         const int c = (k * tpr + t) * VE;
         if (c < dim) {
           if (p > 0) {
             float a[VE];
-            load<float, VE>(cols + c, a);
+            load<float, VE>(cols + c, a, dim - c);
 #pragma unroll
             for (int i = 0; i < VE; ++i) dw[k][i] += a[i];
           }
-          store<float, VE>(p + 1 == per ? out + c : cols + c, dw[k]);
+          if (p + 1 == per) store<float, VE>(out + c, dw[k], dim - c);
+          else store<float, VE>(cols + c, dw[k], dim - c);
         }
       }
     }
@@ -329,7 +365,7 @@ __global__ __launch_bounds__(256) void rms_dw_kernel(
 
 struct Rows {
   long rows;
-  int dim, ve, tpr, block;
+  int dim, tpr, block;
 };
 
 void check_matrix(const torch::Tensor& t, const torch::Tensor& like,
@@ -351,32 +387,12 @@ void check_weight(const torch::Tensor& w, const torch::Tensor& x) {
               "their type or float32, on their GPU");
 }
 
-int narrower(int ve, const torch::Tensor& t) {
-  const int n = vector_width(t.data_ptr(), t.size(-1),
-                             t.dim() == 2 ? t.stride(0) : 0,
-                             t.element_size());
-  return n < ve ? n : ve;
-}
-
-// A weight of fp32 is read by vectors of as many elements as x, at 16 bytes.
-int weight_width(int ve, const torch::Tensor& w) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(w.data_ptr());
-  int n = ve;
-  while (n > 1) {
-    const uintptr_t bytes = n * w.element_size();
-    if (p % (bytes < 16 ? bytes : 16) == 0) break;
-    n /= 2;
-  }
-  return n;
-}
-
-Rows plan(long rows, long dim, int ve) {
+Rows plan(long rows, long dim) {
   TORCH_CHECK(dim >= 1 && dim <= kMaxDim, "rms_norm: rows of 1 to ", kMaxDim,
               " elements, not ", dim);
-  const int held = ve >= 4 ? 4 : ve == 2 ? 8 : 16;
   int tpr = 64;
-  while (tpr * ve * held < dim) tpr *= 4;
-  return Rows{rows, (int)dim, ve, tpr, tpr < 256 ? 256 : tpr};
+  while (tpr * 16 < dim) tpr *= 2;
+  return Rows{rows, (int)dim, tpr, tpr < 256 ? 256 : tpr};
 }
 
 int grid_of(const Rows& r, int most) {
@@ -395,20 +411,15 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fwd(
   check_weight(w, x);
   const c10::DeviceGuard guard(x.device());
   const long rows = x.size(0), dim = x.size(1);
-  int ve = weight_width(narrower(16 / (int)x.element_size(), x), w);
-  if (res) {
-    check_matrix(*res, x, "the residual");
-    ve = narrower(ve, *res);
-  }
-  const Rows r = plan(rows, dim, ve);
+  if (res) check_matrix(*res, x, "the residual");
+  const Rows r = plan(rows, dim);
   auto y = torch::empty({rows, dim}, x.options());
   auto h = torch::empty({res ? rows : 0, dim}, x.options());
   auto rstd = torch::empty({rows}, x.options().dtype(at::kFloat));
   if (rows == 0) return {y, h, rstd};
-  dispatch_vec(x.scalar_type(), ve, "rms_norm", [&](auto t, auto width) {
+  dispatch(x.scalar_type(), "rms_norm", [&](auto t) {
     using T = decltype(t);
-    constexpr int VE = decltype(width)::value;
-    rms_fwd_kernel<T, VE>
+    rms_fwd_kernel<T>
         <<<dim3(grid_of(r, 4096)), dim3(r.block), 0, stream()>>>(
             (const T*)x.data_ptr(), res ? (const T*)res->data_ptr() : nullptr,
             w.data_ptr(), w.scalar_type() == at::kFloat, (T*)y.data_ptr(),
@@ -427,30 +438,21 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fp8(
   check_weight(w, x);
   const c10::DeviceGuard guard(x.device());
   const long rows = x.size(0), dim = x.size(1);
-  const int full = 16 / (int)x.element_size();
-  int ve = weight_width(narrower(full, x), w);
-  if (res) {
-    check_matrix(*res, x, "the residual");
-    ve = narrower(ve, *res);
-  }
+  if (res) check_matrix(*res, x, "the residual");
   TORCH_CHECK(group == 0 || ((group & (group - 1)) == 0 && group >= 16 &&
                              group <= 256 && dim % group == 0),
               "rms_norm_fp8: groups of 16, 32, 64, 128 or 256 columns that "
               "divide the row, not ", group);
-  // a group is joined inside of a wave
-  TORCH_CHECK(group <= 64 * ve, "rms_norm_fp8: rows that are not aligned to "
-              "16 bytes cannot take groups of ", group);
-  const Rows r = plan(rows, dim, ve);
+  const Rows r = plan(rows, dim);
   auto q = torch::empty({rows, dim},
                         x.options().dtype(at::kFloat8_e4m3fn));
   auto scales = torch::empty({rows, group ? dim / group : 1},
                              x.options().dtype(at::kFloat));
   auto h = torch::empty({res ? rows : 0, dim}, x.options());
   if (rows == 0) return {q, scales, h};
-  dispatch_vec(x.scalar_type(), ve, "rms_norm_fp8", [&](auto t, auto width) {
+  dispatch(x.scalar_type(), "rms_norm_fp8", [&](auto t) {
     using T = decltype(t);
-    constexpr int VE = decltype(width)::value;
-    rms_fp8_kernel<T, VE>
+    rms_fp8_kernel<T>
         <<<dim3(grid_of(r, 4096)), dim3(r.block), 0, stream()>>>(
             (const T*)x.data_ptr(), res ? (const T*)res->data_ptr() : nullptr,
             w.data_ptr(), w.scalar_type() == at::kFloat,
@@ -462,42 +464,41 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fp8(
   return {q, scales, h};
 }
 
-// (dh, dw): gy and gh are contiguous, h has contiguous rows.
+// (dh, dw): gy and gh are contiguous, x and the residual have contiguous rows.
 std::tuple<torch::Tensor, torch::Tensor> rms_norm_bwd(
-    torch::Tensor gy, torch::Tensor h, c10::optional<torch::Tensor> gh,
-    torch::Tensor w, torch::Tensor rstd) {
-  check_matrix(h, h, "h");
-  check_matrix(gy, h, "gy");
-  check_weight(w, h);
-  const c10::DeviceGuard guard(h.device());
-  const long rows = h.size(0), dim = h.size(1);
+    torch::Tensor gy, torch::Tensor x, c10::optional<torch::Tensor> res,
+    c10::optional<torch::Tensor> gh, torch::Tensor w, torch::Tensor rstd) {
+  check_matrix(x, x, "x");
+  check_matrix(gy, x, "gy");
+  check_weight(w, x);
+  const c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
   TORCH_CHECK(gy.is_contiguous() && rstd.is_cuda() &&
+              rstd.device() == x.device() &&
               rstd.scalar_type() == at::kFloat && rstd.numel() == rows &&
               rstd.is_contiguous(),
               "rms_norm_bwd: gy contiguous, rstd float32 for each row");
-  int ve = weight_width(narrower(narrower(16 / (int)h.element_size(), h),
-                                 gy), w);
+  if (res) check_matrix(*res, x, "the residual");
   if (gh) {
-    check_matrix(*gh, h, "gh");
+    check_matrix(*gh, x, "gh");
     TORCH_CHECK(gh->is_contiguous(), "rms_norm_bwd: gh contiguous");
-    ve = narrower(ve, *gh);
   }
-  const Rows r = plan(rows, dim, ve);
-  auto dh = torch::empty({rows, dim}, h.options());
+  const Rows r = plan(rows, dim);
+  auto dh = torch::empty({rows, dim}, x.options());
   auto dw = torch::empty({dim}, w.options());
-  const int grid = grid_of(r, 512);  // two of four waves on every CU
-  auto part = torch::empty({grid, dim}, h.options().dtype(at::kFloat));
+  const int grid = grid_of(r, 262144 / r.block);  // four waves on a SIMD
+  auto part = torch::empty({grid, dim}, x.options().dtype(at::kFloat));
   if (rows) {
     const int lds = r.block > r.tpr ? r.dim * (int)sizeof(float) : 0;
-    dispatch_vec(h.scalar_type(), ve, "rms_norm", [&](auto t, auto width) {
+    dispatch(x.scalar_type(), "rms_norm", [&](auto t) {
       using T = decltype(t);
-      constexpr int VE = decltype(width)::value;
-      rms_bwd_kernel<T, VE><<<dim3(grid), dim3(r.block), lds, stream()>>>(
-          (const T*)gy.data_ptr(), (const T*)h.data_ptr(),
+      rms_bwd_kernel<T><<<dim3(grid), dim3(r.block), lds, stream()>>>(
+          (const T*)gy.data_ptr(), (const T*)x.data_ptr(),
+          res ? (const T*)res->data_ptr() : nullptr,
           gh ? (const T*)gh->data_ptr() : nullptr, w.data_ptr(),
           w.scalar_type() == at::kFloat, rstd.data_ptr<float>(),
           (T*)dh.data_ptr(), part.data_ptr<float>(), rows, r.dim,
-          h.stride(0), r.tpr);
+          x.stride(0), res ? res->stride(0) : 0, r.tpr);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }

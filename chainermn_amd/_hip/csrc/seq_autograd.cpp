@@ -18,8 +18,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fwd(
     torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> res,
     double eps);
 std::tuple<torch::Tensor, torch::Tensor> rms_norm_bwd(
-    torch::Tensor gy, torch::Tensor h, c10::optional<torch::Tensor> gh,
-    torch::Tensor w, torch::Tensor rstd);
+    torch::Tensor gy, torch::Tensor x, c10::optional<torch::Tensor> res,
+    c10::optional<torch::Tensor> gh, torch::Tensor w, torch::Tensor rstd);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
     torch::Tensor q, torch::Tensor k, torch::Tensor v,
     torch::Tensor log_decay, c10::optional<torch::Tensor> first,
@@ -95,30 +95,23 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       TORCH_CHECK(res->sizes() == x.sizes(),
                   "rms_norm: the residual has another shape than x");
     const Tensor m = matrix(x);
-    auto [y, h, rstd] = rms_norm_fwd(
-        m, w, res ? c10::optional<Tensor>(matrix(*res)) : c10::nullopt, eps);
-    y = y.view(x.sizes());
-    ctx->saved_data["res"] = res.has_value();
-    if (!res) {
-      ctx->save_for_backward({m, w, rstd});
-      return {y};
-    }
-    h = h.view(x.sizes());
-    ctx->save_for_backward({h, w, rstd});
-    return {y, h};
+    const Tensor r = res ? matrix(*res) : Tensor();
+    auto [y, h, rstd] = rms_norm_fwd(m, w, some(r), eps);
+    ctx->save_for_backward({m, r, w, rstd});
+    if (!res) return {y.view(x.sizes())};
+    return {y.view(x.sizes()), h.view(x.sizes())};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const auto saved = ctx->get_saved_variables();
-    const bool res = ctx->saved_data["res"].toBool();
+    const auto s = ctx->get_saved_variables();
+    const bool res = s[1].defined();
     const Tensor gh = res ? g[1] : Tensor();
     if (!g[0].defined())  // y was not used: the sum's gradient goes on
       return {gh, Tensor(), res ? gh : Tensor(), Tensor()};
-    const Tensor h = matrix(saved[0]);
     auto [dh, dw] = rms_norm_bwd(
-        matrix(g[0]).contiguous(), h,
+        matrix(g[0]).contiguous(), s[0], some(s[1]),
         gh.defined() ? c10::optional<Tensor>(matrix(gh).contiguous())
                      : c10::nullopt,
-        saved[1], saved[2]);
+        s[2], s[3]);
     dh = dh.view(g[0].sizes());
     return {dh, dw, res ? dh : Tensor(), Tensor()};
   }

@@ -10,8 +10,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
     Returns the output, or ``(output, h)`` where there is a residual: ``h``
     is the residual of the next layer.  ``weight`` is of x's type or fp32.
-    Sums are fp32 and each output is rounded once; the backward pass starts
-    from the rounded h.
+    Sums are fp32 and each output and gradient is rounded once.
     """
     check_rms_norm(x, weight, residual)
     if x.is_cuda:

@@ -60,9 +60,8 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, group=None):
     groups = dim // group if group else 1
     if x.is_cuda:
         from chainermn_amd import ops
-        m, r = _rows(x.detach()), None
-        if residual is not None:
-            r = _rows(residual.detach())
+        m = _rows(x.detach())
+        r = None if residual is None else _rows(residual.detach())
         q, scales, h = ops.require().rms_norm_fp8(
             m, weight.detach().contiguous(), r, float(eps), group or 0)
         if x.dim() != 2:
@@ -82,10 +81,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, group=None):
 
 
 def _rows(x):
-    """A matrix of x's rows that can be read by 16 bytes if any copy can."""
+    """A matrix of x's rows, each of them contiguous."""
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    size = x.element_size()
-    if x.stride(1) != 1 or x.stride(0) * size % 16 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return x if x.stride(1) == 1 else x.contiguous()
