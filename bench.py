@@ -63,6 +63,8 @@ def parse_args():
     ap.add_argument('--model', default='resnet50',
                     choices=['resnet50', 'mlp', 'seq2seq'])
     ap.add_argument('--seq-len', type=int, default=64)
+    ap.add_argument('--rnn', default='lstm', choices=['lstm', 'attention'],
+                    help='recurrent layers of seq2seq')
     ap.add_argument('--dtype', default='bf16', choices=['bf16', 'fp32'])
     ap.add_argument('--optimizer', default='sgd',
                     choices=['sgd', 'lars', 'adam'])
@@ -132,7 +134,9 @@ def main():
                         dtype=dtype).to(memory_format=torch.channels_last)
     elif args.model == 'seq2seq':
         from chainermn_amd.models.seq2seq import Seq2Seq
-        model = Seq2Seq(32000, 32000, 1024, n_layers=2).to(device=device)
+        model = Seq2Seq(32000, 32000, 1024, n_layers=2, rnn=args.rnn,
+                        fused_ops=use_gpu and args.rnn != 'lstm'
+                        ).to(device=device)
         xs = torch.randint(2, 32000, (args.batch_size, args.seq_len),
                            device=device)
         ys = torch.randint(2, 32000, (args.batch_size, args.seq_len),

@@ -98,7 +98,7 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
                          double scale, bool has_ignore, long ignore);
 torch::Tensor dropout_fn(torch::Tensor x, torch::Tensor key, long threshold,
                          double scale);
-torch::Tensor dropout_next_key(torch::Tensor state);
+torch::Tensor dropout_next_key(torch::Tensor state, long shift);
 std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor w,
                                     c10::optional<torch::Tensor> res,
                                     double eps);
@@ -124,7 +124,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "dropout from Philox4x32-10, differentiable (no mask is stored)",
         py::call_guard<py::gil_scoped_release>());
   m.def("dropout_next_key", &dropout_next_key,
-        "(seed, call) for one dropout; the state's call number goes up");
+        "(seed + shift, call) for one dropout; the state's call number goes "
+        "up");
   m.def("rms_norm", &rms_norm,
         "[y] or [y, x + residual], differentiable",
         py::call_guard<py::gil_scoped_release>());

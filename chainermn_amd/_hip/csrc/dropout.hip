@@ -74,8 +74,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(
   }
 }
 
-__global__ void dropout_next_key_kernel(long* state, long* key) {
-  key[0] = state[0];
+__global__ void dropout_next_key_kernel(long* state, long* key, long shift) {
+  key[0] = (long)((unsigned long)state[0] + (unsigned long)shift);
   key[1] = state[1];
   state[1] += 1;
 }
@@ -114,12 +114,12 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor key, long threshold,
   return y;
 }
 
-torch::Tensor dropout_next_key(torch::Tensor state) {
+torch::Tensor dropout_next_key(torch::Tensor state, long shift) {
   TORCH_CHECK(is_key(state), "dropout_next_key: two int64 on a GPU");
   const c10::DeviceGuard guard(state.device());
   auto key = torch::empty_like(state);
   dropout_next_key_kernel<<<dim3(1), dim3(1), 0, stream()>>>(
-      state.data_ptr<long>(), key.data_ptr<long>());
+      state.data_ptr<long>(), key.data_ptr<long>(), shift);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return key;
 }

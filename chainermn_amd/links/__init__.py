@@ -8,3 +8,7 @@ from chainermn_amd.links.fused_batch_norm import FusedBNReLU2d  # noqa: F401
 from chainermn_amd.links.batch_normalization import MultiNodeBNReLU2d  # noqa: F401
 from chainermn_amd.links.fused_pool import FusedMaxPool2d  # noqa: F401
 from chainermn_amd.links.fused_conv import FusedConv1x1, FusedConv3x3  # noqa: F401
+from chainermn_amd.links.fused_embedding import FusedEmbedding  # noqa: F401
+from chainermn_amd.links.fused_dropout import FusedDropout  # noqa: F401
+from chainermn_amd.links.fused_rms_norm import FusedRMSNorm  # noqa: F401
+from chainermn_amd.links.linear_attention import LinearAttentionRNN  # noqa: F401,E501

@@ -54,16 +54,21 @@ def dropout_plain(x, key, threshold, scale):
     return torch.where(keep, y, torch.zeros((), dtype=x.dtype))
 
 
-def dropout_next_key(state):
+def dropout_next_key(state, stream=0):
     """The key (seed, call) of one dropout call, from the int64 pair
-    ``state``, whose call number goes up by one.  On the GPU the state is
+    ``state``, whose call number goes up by one.  Each ``stream`` (a rank,
+    for instance) of a state has numbers of its own.  On the GPU the state is
     read and counted there, so a replayed graph draws new numbers."""
     if state.dtype != torch.int64 or state.numel() != 2:
         raise TypeError('dropout: the state is a tensor of two int64 '
                         '(seed, call)')
+    # streams are an odd constant apart, modulo 2^64
+    shift = int(stream) * 0x9E3779B97F4A7C15 & 0xffffffffffffffff
+    shift -= (shift >> 63) << 64
     if state.is_cuda:
         from chainermn_amd import ops
-        return ops.require().dropout_next_key(state)
+        return ops.require().dropout_next_key(state, shift)
     key = state.clone()
+    key[0] += shift
     state[1] += 1
     return key

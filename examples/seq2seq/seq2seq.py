@@ -45,6 +45,11 @@ def main():
     ap.add_argument('--layer', type=int, default=2)
     ap.add_argument('--iterations', type=int, default=100)
     ap.add_argument('--model-parallel', action='store_true')
+    ap.add_argument('--rnn', default='lstm', choices=['lstm', 'attention'],
+                    help='attention = layers of linear attention')
+    ap.add_argument('--dropout', type=float, default=0.0)
+    ap.add_argument('--fused-ops', action='store_true',
+                    help='embedding on its own gfx950 kernels')
     args = ap.parse_args()
 
     chainermn_amd.global_except_hook.add_hook()
@@ -52,7 +57,9 @@ def main():
     device = torch.device('cuda', comm.intra_rank) \
         if torch.cuda.is_available() else torch.device('cpu')
     torch.manual_seed(3)
-    model = Seq2Seq(VOCAB, VOCAB, args.unit, args.layer).to(device)
+    model = Seq2Seq(VOCAB, VOCAB, args.unit, args.layer, rnn=args.rnn,
+                    dropout=args.dropout, fused_ops=args.fused_ops,
+                    comm=comm).to(device)
 
     if args.model_parallel:
         assert comm.size == 2, 'model-parallel demo uses exactly 2 ranks'
