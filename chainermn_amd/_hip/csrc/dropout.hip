@@ -118,6 +118,7 @@ torch::Tensor dropout_next_key(torch::Tensor state, long shift) {
   TORCH_CHECK(is_key(state), "dropout_next_key: two int64 on a GPU");
   const c10::DeviceGuard guard(state.device());
   auto key = torch::empty_like(state);
+  state.unsafeGetTensorImpl()->bump_version();
   dropout_next_key_kernel<<<dim3(1), dim3(1), 0, stream()>>>(
       state.data_ptr<long>(), key.data_ptr<long>(), shift);
   C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -200,7 +200,7 @@ __device__ __forceinline__ void to_frag(const float (&x)[8], frag (&f)[N]) {
 }
 
 // The rows of a chunk between global memory and LDS: a thread's part.  WIDE
-// operands are read by 16 bytes through a buffer resource that ends with the
+// operands are aligned and read through a buffer resource that ends with the
 // last row, so that what lies behind it reads as zero without a branch.
 template <typename T, int D, int C, bool WIDE>
 struct Rows {
@@ -233,9 +233,14 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const T* src = p + (row + i * kStep) * stride + col;
+        const int left = row + i * kStep < n ? cols - col : 0;
+        if (left >= VE) {
+          v[i] = *reinterpret_cast<const typename anywhere<T, VE>::type*>(
+              src);
+        } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          v[i][e] = row + i * kStep < n && col + e < cols ? src[e] : T(0.f);
+          for (int e = 0; e < VE; ++e) v[i][e] = e < left ? src[e] : T(0.f);
+        }
       }
     }
   }
@@ -598,10 +603,9 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
         for (int it = 0; it < 2; ++it) {
           const int i = it * 16 + l;
           if (i >= n) continue;
-          T* dst = op + (c * C + i) * ostride + j;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (j + e < dv) dst[e] = T(o[it][e]);
+          if (j >= dv) continue;
+          const float r[4] = {o[it][0], o[it][1], o[it][2], o[it][3]};
+          store<T, 4>(op + (c * C + i) * ostride + j, r, dv - j);
         }
       }
     }
@@ -921,15 +925,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
   return {o, last, states};
 }
 
-// (dq, dk, dv, dfirst) of the gradients of o and of the last state; dfirst
-// is empty where no state came in.
+// (dq, dk, dv, dfirst) of the gradients of o and of the last state; those
+// that are not needed are not computed, and dfirst is empty then.
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
 linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                      torch::Tensor log_decay,
                      c10::optional<torch::Tensor> first,
                      c10::optional<torch::Tensor> lengths, double scale,
                      torch::Tensor states, torch::Tensor go,
-                     c10::optional<torch::Tensor> glast) {
+                     c10::optional<torch::Tensor> glast, bool need_q,
+                     bool need_k, bool need_v, bool need_first) {
   check_operand(q, q, 4, "q");
   check_operand(k, q, 4, "k");
   check_operand(v, q, 4, "v");
@@ -949,7 +954,8 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   auto gq = torch::empty(q.sizes(), q.options());
   auto gk = torch::empty(k.sizes(), k.options());
   auto gv = torch::empty(v.sizes(), v.options());
-  auto gfirst = torch::empty({first ? b : 0, h, dk, dv}, floats);
+  need_first = need_first && first;
+  auto gfirst = torch::empty({need_first ? b : 0, h, dk, dv}, floats);
   if (b * h == 0) return {gq, gk, gv, gfirst};
   const Cut cut(q, v);
   TORCH_CHECK(states.numel() == cut.states(q) && states.is_contiguous() &&
@@ -966,7 +972,7 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   e.v = operand(go);
   e.out = gv.data_ptr();
   e.first = glast ? glast->data_ptr<float>() : nullptr;
-  e.last = first ? gfirst.data_ptr<float>() : nullptr;
+  e.last = need_first ? gfirst.data_ptr<float>() : nullptr;
   e.states = gstates.data_ptr<float>();
   e.dk = (int)dk;
   e.dv = (int)dv;
@@ -992,13 +998,18 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   a.reverse = false;
   a.inter = c;
   a.gain = 1.f;
-  pr.roles = 1;
-  pr.role[0] = e;
-  if (cut.segments > 1) run_roles(pr, cut, wide, q.scalar_type(), true);
-  pr.roles = 3;
-  pr.role[1] = f;
-  pr.role[2] = a;
-  run_roles(pr, cut, wide, q.scalar_type(), false);
+  // the states before segments are those of the first role
+  const bool backwards = need_k || need_v || need_first;
+  if (cut.segments > 1 && backwards) {
+    pr.roles = 1;
+    pr.role[0] = e;
+    run_roles(pr, cut, wide, q.scalar_type(), true);
+  }
+  pr.roles = 0;
+  if (need_v || need_first) pr.role[pr.roles++] = e;
+  if (need_k) pr.role[pr.roles++] = f;
+  if (need_q) pr.role[pr.roles++] = a;
+  if (pr.roles) run_roles(pr, cut, wide, q.scalar_type(), false);
   return {gq, gk, gv, gfirst};
 }
 
@@ -1020,6 +1031,7 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
   v = rows_of(v);
   auto o = torch::empty({b, h, dv}, q.options());
   if (b * h == 0) return o;
+  state.unsafeGetTensorImpl()->bump_version();
   const bool wide = dv % 4 == 0;
   dispatch(q.scalar_type(), "linear_attention_step", [&](auto t) {
     using T = decltype(t);

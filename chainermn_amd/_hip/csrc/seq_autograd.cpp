@@ -30,12 +30,20 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                      c10::optional<torch::Tensor> first,
                      c10::optional<torch::Tensor> lengths, double scale,
                      torch::Tensor states, torch::Tensor go,
-                     c10::optional<torch::Tensor> glast);
+                     c10::optional<torch::Tensor> glast, bool need_q,
+                     bool need_k, bool need_v, bool need_first);
 
 namespace {
 
 c10::optional<Tensor> some(const Tensor& t) {
   return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt;
+}
+
+// A gradient that is itself to be differentiated would come out as a
+// constant: refused.
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what,
+              ": the gradient is not differentiable (create_graph)");
 }
 
 // A matrix of the rows of x whose rows are contiguous.
@@ -59,6 +67,7 @@ struct EmbedId : torch::autograd::Function<EmbedId> {
     return embed_lookup(ids, w, scale, has_ignore, ignore);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("embed_id");
     Tensor gw;
     if (ctx->needs_input_grad(1))
       gw = embed_grad(ctx->get_saved_variables()[0], g[0].contiguous(),
@@ -79,6 +88,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     return dropout(x.contiguous(), key, threshold, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("dropout");
     return {dropout(g[0].contiguous(), ctx->get_saved_variables()[0],
                     ctx->saved_data["threshold"].toInt(),
                     ctx->saved_data["scale"].toDouble()),
@@ -94,6 +104,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     if (res)
       TORCH_CHECK(res->sizes() == x.sizes(),
                   "rms_norm: the residual has another shape than x");
+    w = w.contiguous();
     const Tensor m = matrix(x);
     const Tensor r = res ? matrix(*res) : Tensor();
     auto [y, h, rstd] = rms_norm_fwd(m, w, some(r), eps);
@@ -102,6 +113,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     return {y.view(x.sizes()), h.view(x.sizes())};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("rms_norm");
     const auto s = ctx->get_saved_variables();
     const bool res = s[1].defined();
     const Tensor gh = res ? g[1] : Tensor();
@@ -132,6 +144,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     return {o, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("linear_attention");
     const auto s = ctx->get_saved_variables();
     const Tensor none;
     if (!g[0].defined() && !g[1].defined())
@@ -141,8 +154,13 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         s[0], s[1], s[2], s[3], some(s[4]), some(s[5]),
         ctx->saved_data["scale"].toDouble(), s[6], go,
         g[1].defined() ? c10::optional<Tensor>(g[1].contiguous())
-                       : c10::nullopt);
-    return {gq, gk, gv, none, s[4].defined() ? gfirst : none, none, none};
+                       : c10::nullopt,
+        ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+        ctx->needs_input_grad(2), s[4].defined() && ctx->needs_input_grad(4));
+    return {ctx->needs_input_grad(0) ? gq : none,
+            ctx->needs_input_grad(1) ? gk : none,
+            ctx->needs_input_grad(2) ? gv : none, none,
+            gfirst.numel() ? gfirst : none, none, none};
   }
 };
 

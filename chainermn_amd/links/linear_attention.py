@@ -68,10 +68,10 @@ class LinearAttentionRNN(nn.Module):
         self.register_buffer('log_decay', -torch.exp(-spread).float(),
                              persistent=False)
 
-    def _apply(self, fn):
+    def _apply(self, fn, recurse=True):
         # a model cast to 16 bits keeps its decays in fp32
         decay = self.log_decay
-        super()._apply(fn)
+        super()._apply(fn, recurse)
         self.log_decay = decay.to(self.log_decay.device)
         return self
 

@@ -56,6 +56,10 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, group=None):
         raise ValueError('rms_norm_fp8: groups of 16, 32, 64, 128 or 256 '
                          'columns that divide the row of {}, not {}'
                          .format(dim, group))
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad
+            or (residual is not None and residual.requires_grad)):
+        raise ValueError('rms_norm_fp8 is not differentiable: use no_grad()')
     shape = x.shape
     groups = dim // group if group else 1
     if x.is_cuda:

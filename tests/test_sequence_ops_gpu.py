@@ -273,7 +273,8 @@ def test_rms_norm(t, rows, dim, residual):
 
 def test_rms_norm_mixed_weight_strides_and_shapes():
     t = torch.bfloat16
-    w = (1 + 0.3 * rand(96, seed=1)).requires_grad_()  # fp32 beside bf16
+    # fp32 beside bf16, every second element of a vector
+    w = (1 + 0.3 * rand(192, seed=1))[::2].detach().requires_grad_()
     big = rand(4, 7, 200, t=t)
     for x in (big[..., :96], big[..., 3:99], big.transpose(0, 1)[..., :96],
               rand(4, 96, 7, t=t).transpose(1, 2),
@@ -451,6 +452,57 @@ def test_linear_attention_heads_of_one_projection():
     assert torch.equal(g, torch.stack(torch.autograd.grad(o2, parts, go), 2))
 
 
+def test_linear_attention_shared_and_broadcast_inputs():
+    b, n, h, d = 2, 75, 4, 32
+    q, k, v = (rand(b, n, x, d, seed=x) for x in (h, 1, 2))
+    s0 = rand(1, h, d, d, seed=9)
+    go = rand(b, n, h, d, seed=5)
+    ld = torch.linspace(-1, -0.01, h, device=DEV)
+
+    def run(expand):
+        ins = [x.clone().requires_grad_() for x in (q, k, v, s0)]
+        o, s = functions.linear_attention(*expand(*ins[:3]), ld,
+                                          initial_state=ins[3].expand(
+                                              b, -1, -1, -1))
+        return [o.detach(), s.detach()] + list(torch.autograd.grad(
+            (o, s), ins, (go, torch.ones_like(s))))
+
+    # one head of k and two of v for four of q, as views and as copies
+    views = run(lambda q, k, v: (q, k.expand(-1, -1, h, -1),
+                                 v.unsqueeze(3).expand(-1, -1, -1, 2, -1)
+                                 .flatten(2, 3)))
+    copies = run(lambda q, k, v: (q, k.repeat(1, 1, h, 1),
+                                  v.repeat_interleave(2, 2)))
+    for x, y in zip(views, copies):
+        # the same kernels on the same values; only torch's sums over the
+        # shared heads may differ in their order, by 4 terms
+        assert (x - y).abs().max() <= 8 * E * y.abs().max()
+    # a gradient that is one value everywhere
+    ins = [x.requires_grad_() for x in (q, k.repeat(1, 1, h, 1),
+                                        v.repeat_interleave(2, 2))]
+    o, _ = functions.linear_attention(*ins, ld)
+    a = torch.autograd.grad(o.sum(), ins, retain_graph=True)
+    for x, y in zip(a, torch.autograd.grad(o, ins, torch.ones_like(o))):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize('length', [40, 600])
+def test_linear_attention_some_of_the_gradients(length):
+    ins = [rand(1, length, 2, 64, seed=i).requires_grad_() for i in range(3)]
+    s0 = rand(1, 2, 64, 64, seed=4).requires_grad_()
+    ld = torch.tensor([-0.3, -0.002], device=DEV)
+    o, s = functions.linear_attention(*ins, ld, initial_state=s0)
+    go = rand(*o.shape, seed=7)
+    every = torch.autograd.grad(o, ins + [s0], go, retain_graph=True)
+    for i, x in enumerate(ins + [s0]):
+        g, = torch.autograd.grad(o, x, go, retain_graph=True)
+        assert torch.equal(g, every[i])
+    # a state that is not trained
+    o, s = functions.linear_attention(*ins, ld, initial_state=s0.detach())
+    for a, b in zip(torch.autograd.grad(o, ins, go), every):
+        assert torch.equal(a, b)
+
+
 def test_linear_attention_behind_the_end_nothing_is_read():
     for bad in (float('nan'), float('inf'), torch.finfo(torch.float32).min):
         q, k, v = (rand(2, 100, 2, 32, seed=i) for i in range(3))
@@ -608,9 +660,50 @@ def test_operators_in_a_graph():
         assert torch.equal(eager[0].detach(), want[0])
 
 
+def test_second_derivatives_are_refused():
+    x = rand(2, 3, 2, 8).requires_grad_()
+    ld, w = torch.zeros(2, device=DEV), torch.ones(8, device=DEV)
+    ids = torch.tensor([0, 1], device=DEV)
+    for y in (functions.linear_attention(x, x, x, ld)[0],
+              functions.rms_norm(x, w), functions.dropout(x, key_of(1, 2)),
+              functions.embed_id(ids, x.view(12, 8))):
+        with pytest.raises(RuntimeError, match='not differentiable'):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_what_is_updated_in_place_says_so():
+    state = torch.zeros(2, 2, 8, 8, device=DEV)
+    x = rand(2, 2, 8)
+    before = state._version
+    ops.linear_attention_step(x, x, x, state, torch.zeros(2, device=DEV))
+    assert state._version > before
+    key = key_of(1, 2)
+    before = key._version
+    ops.dropout_next_key(key, stream=3)
+    assert key._version > before
+    assert torch.equal(ops.dropout_next_key(key, stream=3).cpu(),
+                       ops.dropout_next_key(torch.tensor([1, 3]), stream=3))
+
+
+def test_rms_norm_fp8_of_what_is_not_finite():
+    x = rand(3, 64)
+    x[1, 5] = float('nan')
+    q, scales = ops.rms_norm_fp8(x, torch.ones(64, device=DEV))
+    assert torch.isnan(q[1].float()).all()
+    assert torch.isfinite(q[::2].float()).all()
+    w = torch.ones(64, device=DEV)
+    w[7] = float('nan')
+    q, scales = ops.rms_norm_fp8(rand(2, 64), w, group=32)
+    bad = torch.isnan(q.float())
+    assert bad[:, 7].all() and bad.sum() == 2 and torch.isfinite(scales).all()
+
+
 def test_refusals_on_the_gpu():
     ld = torch.zeros(2, device=DEV)
     x = rand(2, 3, 2, 8)
+    with pytest.raises(ValueError, match='not differentiable'):
+        ops.rms_norm_fp8(rand(2, 8).requires_grad_(), torch.ones(
+            8, device=DEV))
     double = x.double()
     with pytest.raises(RuntimeError, match='float32'):
         functions.linear_attention(double, double, double, ld)
