@@ -394,25 +394,22 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
   // the state: tile t has rows 16t + 4g + r of dk, column col0 + l of dv
   const int col0 = wave * 16;
   acc4 s[KT];
-  bool some = false;  // whether the state can be other than zero
+  bool some = true;  // whether the state can be other than zero
   float* stored = ro.states + ((long)bh * pr.segments + seg) * (D * D);
   // byte offset of an element of an end's state
   auto offset = [&](int i, int j) {
     const int at = ro.turned ? j * dk + i : i * dv + j;
     return i < dk && j < dv ? at * 4 : kBehind;
   };
-  if (seg == entry) {
-    some = ro.first != nullptr;
-    const auto rsrc = buffer(ro.first + (some ? (long)bh * dk * dv : 0),
-                             some ? dk * dv * 4 : 0);
+  if (seg == entry && ro.first) {
+    const auto rsrc = buffer(ro.first + (long)bh * dk * dv, dk * dv * 4);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         s[t][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
             rsrc, offset(t * 16 + 4 * g + r, col0 + l), 0, 0));
-  } else if constexpr (OUT) {
-    some = true;
+  } else if (OUT && seg != entry) {
     if (ro.turned) {  // stored for the transposed state: row and column swap
 #pragma unroll
       for (int t = 0; t < KT; ++t)
@@ -427,6 +424,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
                                               threadIdx.x * 4);
     }
   } else {
+    some = false;
 #pragma unroll
     for (int t = 0; t < KT; ++t) s[t] = acc4{0.f, 0.f, 0.f, 0.f};
   }
