@@ -445,6 +445,17 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
   if constexpr (!OUT) {
     if (some) decay_state(expm1f(ld * live));
   }
+  // Three waves have a tile of scores each, (0, 0), (1, 1) and the one between
+  // them, and the factors of its elements; zero where the mask is.
+  const int it = rev ? wave == 1 : wave > 0;
+  const int jt = rev ? wave > 0 : wave == 1;
+  float fade[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = it * 16 + l, j = jt * 16 + 4 * g + r;
+    const int d = rev ? j - i : i - j;
+    fade[r] = d >= 0 ? ro.intra * power(log2, d) : 0.f;
+  }
   int of_tables = 0;   // the n that tables and `less` are for
   float less = 0.f;    // lam^n - 1, which keeps a decay near one exact
   auto chunk = [&](int step, auto slot) {
@@ -475,11 +486,8 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
 
     acc4 o[2] = {acc4{0.f, 0.f, 0.f, 0.f}, acc4{0.f, 0.f, 0.f, 0.f}};
     if constexpr (OUT) {
-      // scores, transposed: rows j, columns i; the tiles (0, 0), (1, 1) and
-      // the one between them
+      // scores, transposed: rows j, columns i
       if (wave < 3) {
-        const int it = rev ? wave == 1 : wave > 0;
-        const int jt = rev ? wave > 0 : wave == 1;
         acc4 p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -495,11 +503,8 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
         }
         unsigned term[4][NI];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = it * 16 + l, j = jt * 16 + 4 * g + r;
-          const int d = rev ? j - i : i - j;
-          cut<NI>(d >= 0 ? p[r] * (ro.intra * power(log2, d)) : 0.f, term[r]);
-        }
+        for (int r = 0; r < 4; ++r)
+          cut<NI>(fade[r] != 0.f ? p[r] * fade[r] : 0.f, term[r]);
 #pragma unroll
         for (int x = 0; x < NI; ++x)
           *reinterpret_cast<uint2*>(
