@@ -449,6 +449,61 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(
   }
 }
 
+// The whole gradient of a few tokens and rows in one launch: a workgroup looks
+// for its row among all ids, each wave in a run of them.
+// grid: (vocab, slices).
+template <typename T, typename I>
+__global__ __launch_bounds__(kSplitThreads) void embed_direct_kernel(
+    const I* __restrict__ ids, const T* __restrict__ gy, T* __restrict__ dw,
+    long n, long dim, bool has_ignore, long ignore, float scale) {
+  constexpr int VE = kWidth<T>;
+  __shared__ float part[kSplitWaves][64 * VE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = blockIdx.x, col0 = blockIdx.y * 64l * VE;
+  const long col = column<VE>(col0 + lane * VE, dim);
+  float acc[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  const long per = (n + kSplitThreads - 1) / kSplitThreads * 64;
+  const long first = wave * per, last = first + per < n ? first + per : n;
+  if (!(has_ignore && row == ignore)) {
+    for (long p0 = first; p0 < last; p0 += 64) {
+      const bool is = p0 + lane < last && ids[p0 + lane] == row;
+      unsigned long long left = __ballot(is);
+      while (left) {
+        constexpr int U = 4;  // rows in flight
+        float g[U][VE];
+        int found = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int at = __ffsll(left) - 1;
+          if (at >= 0) {
+            load<T, VE>(gy + (p0 + at) * dim + col, g[u], dim);
+            left &= left - 1;
+            ++found;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < found)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) acc[i] += g[u][i];
+      }
+    }
+  }
+  // a row's odd end is moved onto the vector before it, here too
+#pragma unroll
+  for (int i = 0; i < VE; ++i)
+    if (col - col0 + i >= lane * VE) part[wave][col - col0 + i] = acc[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 64 * VE && col0 + c < dim;
+       c += kSplitThreads) {
+    float sum = 0.f;
+    for (int w = 0; w < kSplitWaves; ++w) sum += part[w][c];
+    dw[row * dim + col0 + c] = T(sum * scale);
+  }
+}
+
 void check_ids(const torch::Tensor& ids, const char* what) {
   TORCH_CHECK(ids.is_cuda() && ids.is_contiguous() &&
               (ids.scalar_type() == at::kLong ||
@@ -508,6 +563,27 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
   const c10::DeviceGuard guard(gy.device());
   const long dim = gy.size(-1);
   auto dw = torch::empty({vocab, dim}, gy.options());
+  const int ve = 16 / (int)gy.element_size();
+  const int slices = int((dim + 64 * ve - 1) / (64 * ve));
+  // A row of the table for each workgroup, while there are no more than run
+  // at once and no more tokens than a wave finds quickly.  (1280 tokens of 64
+  // x 512 in fp32: 5 us instead of 22 us.)
+  if (vocab * slices <= 1024 && n <= 4096) {
+    dispatch(gy.scalar_type(), "embed_grad", [&](auto t) {
+      using T = decltype(t);
+      auto go = [&](auto i) {
+        using I = decltype(i);
+        embed_direct_kernel<T, I>
+            <<<dim3(vocab, slices), dim3(kSplitThreads), 0, stream()>>>(
+                (const I*)ids.data_ptr(), (const T*)gy.data_ptr(),
+                (T*)dw.data_ptr(), n, dim, has_ignore, ignore, (float)scale);
+      };
+      if (ids.scalar_type() == at::kLong) go(long());
+      else go(int());
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    return dw;
+  }
   // 256 buckets, or as many as leave 1024 ids to each; above 2^19 ids a
   // bucket is sorted in parts
   int bucket_bits = 0;
@@ -552,8 +628,6 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
       order, sorted, range, tokens);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 
-  const int ve = 16 / (int)gy.element_size();
-  const int slices = int((dim + 64 * ve - 1) / (64 * ve));
   // sorted tokens of a wave: 32, or fewer until four waves have work on each
   // SIMD (22500 rows of 1520 bytes at 16: 32 us, at 32: 35 us)
   int size = 32;

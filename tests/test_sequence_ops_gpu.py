@@ -72,7 +72,7 @@ def embed_case(ids, W, gy, scale, ignore):
 @pytest.mark.parametrize('vocab,dim,tokens', [
     (1, 1, 1), (1, 7, 33), (2, 8, 31), (64, 512, 1280), (5, 64, 4097),
     (1000, 33, 32), (3000, 100, 2049), (300000, 8, 1500), (257, 1030, 777),
-    (1100000, 3, 5000), (700, 5, 70000)])
+    (1100000, 3, 5000), (700, 5, 70000), (5000, 40, 1), (2000, 513, 33)])
 def test_embed(t, vocab, dim, tokens):
     g = torch.Generator(device=DEV).manual_seed(tokens)
     ids = torch.randint(0, vocab, (tokens,), generator=g, device=DEV)
@@ -83,12 +83,14 @@ def test_embed(t, vocab, dim, tokens):
                2.5, -1)
 
 
+@pytest.mark.parametrize('vocab', [40, 3000])
 @pytest.mark.parametrize('tokens', [1, 32, 33, 64, 5000])
-def test_embed_all_the_same_id(tokens):
+def test_embed_all_the_same_id(vocab, tokens):
     ids = torch.full((tokens,), 17, device=DEV, dtype=torch.int32)
-    embed_case(ids, rand(40, 96), rand(tokens, 96, seed=1), -0.5, None)
+    embed_case(ids, rand(vocab, 96), rand(tokens, 96, seed=1), -0.5, None)
     # and all ignored: the gradient is zero
-    _, dW = embed_case(ids, rand(40, 96), rand(tokens, 96, seed=1), 1.0, 17)
+    _, dW = embed_case(ids, rand(vocab, 96), rand(tokens, 96, seed=1), 1.0,
+                       17)
     assert not dW.any()
 
 
