@@ -36,7 +36,8 @@ class LinearAttentionRNN(nn.Module):
     n_heads, d, d]`` in fp32 with ``d = hidden_size / n_heads`` (at most 128).
     ``lengths`` are those of a padded batch.  The heads' memories, after which
     a token's weight has fallen to 1/e, are spread from ``memory[0]`` to
-    ``memory[1]`` tokens and are not learned.
+    ``memory[1]`` tokens and are not learned.  Under autocast the sum of the
+    layers keeps the type of ``x``.
     """
 
     def __init__(self, input_size, hidden_size, num_layers=1, n_heads=None,
@@ -80,12 +81,12 @@ class LinearAttentionRNN(nn.Module):
         if state is not None and state.shape[0] != len(self.layers):
             raise ValueError('LinearAttentionRNN: a state of {} layers, not '
                              '{}'.format(state.shape[0], len(self.layers)))
-        h, branch, last = self.project(x), None, []
+        h, branch, last = self.project(x).to(x.dtype), None, []
         for i, layer in enumerate(self.layers):
             if branch is None:
                 y = layer.norm(h)
             else:
-                y, h = layer.norm(branch, residual=h)
+                y, h = layer.norm(branch.to(h.dtype), residual=h)
             q, k, v = layer.qkv(y).view(
                 b, t, 3, self.n_heads, self.head).unbind(2)
             o, s = functions.linear_attention(
@@ -95,7 +96,7 @@ class LinearAttentionRNN(nn.Module):
             last.append(s)
             o = layer.head_norm(o).flatten(2)
             branch = layer.dropout(layer.out(o))
-        y, _ = self.norm(branch, residual=h)
+        y, _ = self.norm(branch.to(h.dtype), residual=h)
         return y, torch.stack(last)
 
     @torch.no_grad()
@@ -103,14 +104,14 @@ class LinearAttentionRNN(nn.Module):
         """One token for each sequence: ``x [batch, input_size]``, and the
         state of ``forward``, which is updated in place."""
         b = x.shape[0]
-        h, branch = self.project(x), None
+        h, branch = self.project(x).to(x.dtype), None
         for i, layer in enumerate(self.layers):
             if branch is None:
                 y = layer.norm(h)
             else:
-                y, h = layer.norm(branch, residual=h)
+                y, h = layer.norm(branch.to(h.dtype), residual=h)
             q, k, v = layer.qkv(y).view(
                 b, 3, self.n_heads, self.head).unbind(1)
             o = ops.linear_attention_step(q, k, v, state[i], self.log_decay)
             branch = layer.out(layer.head_norm(o).flatten(1))
-        return self.norm(branch, residual=h)[0]
+        return self.norm(branch.to(h.dtype), residual=h)[0]

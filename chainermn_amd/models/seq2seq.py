@@ -114,15 +114,17 @@ class Seq2Seq(nn.Module):
         ``[batch, max_length]`` tokens that follow ``bos``."""
         training = self.training
         self.eval()
-        state = self.encoder(xs, lengths)
-        y = torch.full((xs.shape[0],), bos, dtype=torch.long,
-                       device=xs.device)
-        out = []
-        for _ in range(max_length):
-            logits, state = self.decoder.step(y, state)
-            y = logits.argmax(-1)
-            out.append(y)
-        self.train(training)
+        try:
+            state = self.encoder(xs, lengths)
+            y = torch.full((xs.shape[0],), bos, dtype=torch.long,
+                           device=xs.device)
+            out = []
+            for _ in range(max_length):
+                logits, state = self.decoder.step(y, state)
+                y = logits.argmax(-1)
+                out.append(y)
+        finally:
+            self.train(training)
         return torch.stack(out, 1) if out else xs.new_empty(
             (xs.shape[0], 0), dtype=torch.long)
 

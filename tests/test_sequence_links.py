@@ -144,6 +144,25 @@ def test_seq2seq_trains_and_translates(rnn):
     assert torch.equal(logits.argmax(-1), out)
 
 
+def test_attention_rnn_under_autocast():
+    rnn = _rnn()
+    x = torch.randn(2, 5, 6, requires_grad=True)
+    with torch.autocast('cpu', dtype=torch.bfloat16):
+        y, state = rnn(x)
+        one = rnn.step(x[:, 0], torch.zeros_like(state))
+    # 16-bit products between an fp32 sum of layers and fp32 states
+    assert y.dtype == one.dtype == state.dtype == torch.float32
+    y.sum().backward()
+    assert torch.isfinite(x.grad).all() and x.grad.any()
+
+
+def test_translate_leaves_the_mode_as_it_was():
+    model = Seq2Seq(20, 20, 16, 1, rnn='attention')
+    with pytest.raises(IndexError):
+        model.translate(torch.tensor([[1, 99]]), 3)
+    assert model.training
+
+
 def _mp_worker(rank, size):
     comm = chainermn_amd.create_communicator('naive')
     torch.manual_seed(1)
@@ -240,3 +259,17 @@ def test_seq2seq_on_a_gpu_is_what_it_is_on_the_cpu(rnn):
     top = logits.topk(2, -1)
     clear = (top.values[..., 0] - top.values[..., 1]) > 1e-4
     assert torch.equal(out[clear], top.indices[..., 0][clear])
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason='needs ROCm GPU')
+def test_attention_rnn_under_autocast_on_a_gpu():
+    torch.manual_seed(1)
+    rnn = links.LinearAttentionRNN(64, 128, num_layers=2).cuda()
+    x = torch.randn(3, 40, 64, device='cuda', requires_grad=True)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        y, state = rnn(x)
+        one = rnn.step(x[:, 0], torch.zeros_like(state))
+    assert y.dtype == one.dtype == state.dtype == torch.float32
+    y.sum().backward()
+    assert torch.isfinite(x.grad).all() and x.grad.any()
