@@ -6,7 +6,8 @@ from chainermn_amd.ops._embedding import check_embedding, embed_plain
 
 def embed_id(x, W, ignore_label=None, scale=1.0):
     """``scale * W[x]``: ``x`` int32 or int64 of any shape, ``W``
-    ``[vocabulary, units]``; returns ``x.shape + (units,)`` in W's type.
+    ``[vocabulary, units]`` with contiguous rows; returns
+    ``x.shape + (units,)`` in W's type.
 
     An id equal to ``ignore_label`` (any number, -1 or 0 for instance) gives
     a row of zeros and no gradient.  Any other id outside of the vocabulary

@@ -15,7 +15,8 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None,
     ``[heads]`` fp32, at most zero, not differentiable; ``initial_state``
     ``[batch, heads, dk, dv]`` fp32, zero by default; ``scale`` is
     ``dk ** -0.5`` by default.  ``lengths`` (int32 or int64, ``[batch]``)
-    are the sequences' lengths in a padded batch: what lies behind them is
+    are the sequences' lengths in a padded batch, taken as 0 to ``length``
+    where they lie outside of it: what lies behind them is
     not read, the output there is zero, and the state stops at the last
     token.
 
@@ -36,7 +37,10 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None,
     if q.is_cuda:
         if initial_state is not None:
             initial_state = initial_state.contiguous()
+        if lengths is not None:
+            lengths = lengths.contiguous()
         return tuple(ops.require().linear_attention(
-            q, k, v, log_decay, initial_state, lengths, float(scale)))
+            q, k, v, log_decay.contiguous(), initial_state, lengths,
+            float(scale)))
     return attention_plain(q, k, v, log_decay, initial_state, lengths,
                            float(scale))

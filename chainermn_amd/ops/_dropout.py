@@ -5,6 +5,8 @@ Kernels: _hip/csrc/dropout.hip.
 
 import torch
 
+from chainermn_amd.ops._embedding import wide
+
 _M = 0xffffffff
 
 
@@ -50,7 +52,7 @@ def philox_words(key, n):
 
 def dropout_plain(x, key, threshold, scale):
     keep = (philox_words(key, x.numel()) >= threshold).view(x.shape)
-    y = (x.float() * scale).to(x.dtype)
+    y = (wide(x) * scale).to(x.dtype)
     return torch.where(keep, y, torch.zeros((), dtype=x.dtype))
 
 

@@ -7,7 +7,10 @@ Kernels: _hip/csrc/embed.hip.  The reference's model used Chainer's EmbedID
 import torch
 import torch.nn.functional as F
 
-FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+def wide(x):
+    """What the plain forms compute in: fp32, or fp64 for fp64."""
+    return x if x.dtype == torch.float64 else x.float()
 
 
 def check_embedding(ids, W):
@@ -29,5 +32,5 @@ def embed_plain(ids, W, ignore_label, scale):
         at = at.masked_fill(skip, 0)
     y = F.embedding(at, W)
     if scale != 1.0:
-        y = (y.float() * scale).to(W.dtype)
+        y = (wide(y) * scale).to(W.dtype)
     return y if skip is None else y.masked_fill(skip[..., None], 0)

@@ -6,6 +6,8 @@ Kernels: _hip/csrc/linear_attention.hip.
 
 import torch
 
+from chainermn_amd.ops._embedding import wide
+
 MAX_HEAD = 128
 
 
@@ -48,12 +50,15 @@ def attention_plain(q, k, v, log_decay, first, lengths, scale):
     if lengths is None:
         n = torch.full((q.shape[0],), t, device=q.device)
     else:
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError('linear_attention: lengths must be int32 or '
+                            'int64, not {}'.format(lengths.dtype))
         n = lengths.long().clamp(0, t)
     live = (pos < n[:, None])[:, :, None, None]
     zero = torch.zeros((), device=q.device)
-    qf, kf, vf = (torch.where(live, x.float(), zero).transpose(1, 2)
-                  for x in (q, k, v))
-    ld = log_decay.clamp(min=-200.0)[:, None]  # 0 * log(0) is 0 here
+    qf, kf, vf = (torch.where(live, wide(x), zero.to(wide(x).dtype))
+                  .transpose(1, 2) for x in (q, k, v))
+    ld = log_decay.clamp(min=-200.0)[:, None].to(qf.dtype)  # 0 * log(0) is 0
     gap = pos[:, None] - pos
     w = torch.where(gap >= 0, torch.exp(
         gap.clamp(min=0) * ld[:, :, None]), zero)
@@ -61,10 +66,11 @@ def attention_plain(q, k, v, log_decay, first, lengths, scale):
     left = (n[:, None, None] - 1 - pos).clamp(min=0)
     last = kf.transpose(-1, -2) @ (vf * torch.exp(left * ld)[..., None])
     if first is not None:
+        first = first.to(qf.dtype)
         o = o + (qf @ first) * torch.exp((pos + 1) * ld)[..., None]
         last = last + first * torch.exp(
             n[:, None, None, None] * ld[..., None])
-    return (o * scale).transpose(1, 2).to(q.dtype), last
+    return (o * scale).transpose(1, 2).to(q.dtype), last.float()
 
 
 def linear_attention_step(q, k, v, state, log_decay, scale=None):
@@ -88,8 +94,8 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None):
                          'functions.linear_attention, or no_grad()')
     if q.is_cuda:
         from chainermn_amd import ops
-        return ops.require().linear_attention_step(q, k, v, state, log_decay,
-                                                   float(scale))
+        return ops.require().linear_attention_step(
+            q, k, v, state, log_decay.contiguous(), float(scale))
     if not state.is_contiguous():
         raise ValueError('linear_attention: a state is contiguous')
     state.mul_(torch.exp(log_decay)[:, None, None]).add_(

@@ -6,6 +6,8 @@ Kernels: _hip/csrc/rms_norm.hip.
 
 import torch
 
+from chainermn_amd.ops._embedding import wide
+
 E4M3_MAX = 448.0
 MAX_DIM = 16384
 
@@ -31,12 +33,12 @@ def check_rms_norm(x, weight, residual):
 
 
 def rms_plain(x, weight, residual, eps):
-    """(y, h) in fp32 and not yet rounded."""
-    h = x.float()
+    """(y, h), not yet rounded."""
+    h = wide(x)
     if residual is not None:
-        h = h + residual.float()
+        h = h + wide(residual)
     y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
-    return y * weight.float(), h
+    return y * wide(weight), h
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6, group=None):

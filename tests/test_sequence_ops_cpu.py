@@ -177,3 +177,27 @@ def test_refusals():
     for ratio in (1.0, -0.1, float('nan')):
         with pytest.raises(ValueError, match='ratio'):
             functions.dropout(W, key_of(0, 0), ratio=ratio)
+
+
+def test_float64_stays_float64():
+    torch.manual_seed(0)
+    x = torch.randn(3, 4, 2, 8, dtype=torch.float64, requires_grad=True)
+    w = torch.randn(8, dtype=torch.float64, requires_grad=True)
+    ld = torch.tensor([-0.3, -0.1])
+    # fp32 anywhere would be off by more than 1e-9 of differences of 1e-6
+    assert torch.autograd.gradcheck(
+        lambda x, w: functions.rms_norm(x, w, residual=x)[0], (x, w))
+    assert torch.autograd.gradcheck(
+        lambda x: functions.dropout(x, key_of(1, 2), ratio=0.3), (x,))
+    assert torch.autograd.gradcheck(
+        lambda x: functions.linear_attention(x, x, x, ld)[0], (x,))
+    ids = torch.tensor([0, 2, -1, 2])
+    assert torch.autograd.gradcheck(
+        lambda W: functions.embed_id(ids, W, ignore_label=-1, scale=3.0),
+        (torch.randn(3, 4, dtype=torch.float64, requires_grad=True),))
+
+
+def test_lengths_of_another_type_are_refused():
+    x, ld = torch.randn(2, 3, 2, 8), torch.zeros(2)
+    with pytest.raises(TypeError, match='lengths'):
+        functions.linear_attention(x, x, x, ld, lengths=torch.ones(2))
