@@ -44,18 +44,12 @@ __device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2,
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(
     const T* __restrict__ x, T* __restrict__ y, const long* __restrict__ key,
-    long n, unsigned threshold, float scale, bool aligned) {
+    long n, unsigned threshold, float scale) {
   const unsigned long seed = key[0], call = key[1];
   const long stride = gridDim.x * 256l * 8;
   for (long i = (blockIdx.x * 256l + threadIdx.x) * 8; i < n; i += stride) {
-    const bool whole = aligned && i + 8 <= n;
     float r[8];
-    if (whole) {
-      load<T, 8>(x + i, r);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = i + j < n ? float(x[i + j]) : 0.f;
-    }
+    load<T, 8>(x + i, r, n - i);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const unsigned long block = (unsigned long)i / 4 + h;
@@ -67,13 +61,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(
       for (int j = 0; j < 4; ++j)
         r[4 * h + j] = word[j] >= threshold ? r[4 * h + j] * scale : 0.f;
     }
-    if (whole) {
-      store<T, 8, true>(y + i, r);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i + j < n) y[i + j] = T(r[j]);
-    }
+    store<T, 8, true>(y + i, r, n - i);
   }
 }
 
@@ -102,7 +90,6 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor key, long threshold,
   auto y = torch::empty_like(x);
   const long n = x.numel();
   if (n == 0) return y;
-  const bool aligned = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   long blocks = (n + 2047) / 2048;
   // the rest by strides of the grid (2^27 elements of bf16, both passes: 207
   // us; with a workgroup for every 2048, 218 us)
@@ -111,7 +98,7 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor key, long threshold,
     using T = decltype(t);
     dropout_kernel<T><<<dim3(blocks), dim3(256), 0, stream()>>>(
         (const T*)x.data_ptr(), (T*)y.data_ptr(), key.data_ptr<long>(), n,
-        (unsigned)threshold, (float)scale, aligned);
+        (unsigned)threshold, (float)scale);
   });
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return y;

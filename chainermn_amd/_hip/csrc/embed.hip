@@ -529,16 +529,16 @@ torch::Tensor embed_lookup(torch::Tensor ids, torch::Tensor w, double scale,
               "contiguous rows on the ids' GPU");
   const c10::DeviceGuard guard(w.device());
   const long n = ids.numel(), dim = w.size(1);
-  auto shape = ids.sizes().vec();
-  shape.push_back(dim);
-  auto y = torch::empty(shape, w.options());
-  if (n == 0) return y;
   const int ve = 16 / (int)w.element_size();
   const long nvec = (dim + ve - 1) / ve;
   int lanes = 64;  // of a row; a wave takes several short ones
   while (lanes > 1 && lanes / 2 >= nvec) lanes /= 2;
   const long blocks = (n + 256 / lanes - 1) / (256 / lanes);
-  TORCH_CHECK(blocks < (1l << 31), "embed_lookup: too many tokens");
+  check_grid(blocks, 256, "embed_lookup");
+  auto shape = ids.sizes().vec();
+  shape.push_back(dim);
+  auto y = torch::empty(shape, w.options());
+  if (n == 0) return y;
   dispatch(w.scalar_type(), "embed_lookup", [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto i) {
@@ -645,8 +645,8 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
   float* tail = head + (long)chunks * dim;
   const long zero_waves = vocab < 4096 ? vocab : 4096;
   const long blocks = ((long)chunks * slices + zero_waves + 3) / 4;
-  TORCH_CHECK(blocks < (1l << 31) && slices < 65536,
-              "embed_grad: too many elements");
+  check_grid(blocks, 256, "embed_grad");
+  TORCH_CHECK(slices < 65536, "embed_grad: rows of too many elements");
   dispatch(gy.scalar_type(), "embed_grad", [&](auto t) {
     using T = decltype(t);
     embed_rows_kernel<T><<<dim3(blocks), dim3(256), 0, stream()>>>(

@@ -697,8 +697,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Problem pr,
 }
 
 // One token: the state is read, updated in place and written, and bounds the
-// kernel (64 sequences, 16 heads of 64: 7.4 us, 4.6 TB/s).  A workgroup has 16 * VE columns of the state of a sequence and
-// head; a thread has VE of them in every 16th row.
+// kernel (64 sequences, 16 heads of 64: 7.4 us, 4.6 TB/s).  A workgroup has
+// 16 * VE columns of the state of a sequence and head; a thread has VE of
+// them in every 16th row.
 template <typename T, int VE>
 __global__ __launch_bounds__(kThreads) void step_kernel(
     const T* __restrict__ q, const T* __restrict__ k,
@@ -871,9 +872,10 @@ void run_roles(const Problem& pr, const Cut& cut, bool wide, at::ScalarType t,
 Problem problem(const torch::Tensor& q, const torch::Tensor& log_decay,
                 const c10::optional<torch::Tensor>& lengths, const Cut& cut) {
   Problem pr{};
-  TORCH_CHECK(q.size(1) < (1l << 30) && q.size(0) * q.size(2) < (1l << 28),
+  // three roles of 512 threads each stay below the 2^32 of a launch
+  TORCH_CHECK(q.size(1) < (1l << 30) && q.size(0) * q.size(2) < (1l << 21),
               "linear_attention: fewer than 2^30 tokens of a sequence and "
-              "2^28 sequences times heads");
+              "2^21 sequences times heads");
   pr.batch = (int)q.size(0);
   pr.length = (int)q.size(1);
   pr.heads = (int)q.size(2);
@@ -1047,6 +1049,7 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
   v = rows_of(v);
   auto o = torch::empty({b, h, dv}, q.options());
   if (b * h == 0) return o;
+  check_grid(b * h, kThreads, "linear_attention_step");
   state.unsafeGetTensorImpl()->bump_version();
   const bool wide = dv % 4 == 0;
   dispatch(q.scalar_type(), "linear_attention_step", [&](auto t) {

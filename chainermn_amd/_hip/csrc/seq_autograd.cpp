@@ -3,6 +3,7 @@
 // than the smaller of these kernels.
 
 #include <torch/extension.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 using torch::Tensor;
 using torch::autograd::AutogradContext;
@@ -39,11 +40,28 @@ c10::optional<Tensor> some(const Tensor& t) {
   return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt;
 }
 
-// A gradient that is itself to be differentiated would come out as a
-// constant: refused.
+// At the beginning of each backward pass.  A gradient that is itself to be
+// differentiated would come out as a constant: refused.  So is one that is
+// captured into a graph for a leaf whose gradients are summed on the default
+// stream, since an eager graph of it lives: that stream would have to wait
+// for the captured one, which ends the process.
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what,
               ": the gradient is not differentiable (create_graph)");
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() ==
+      c10::hip::CaptureStatus::None)
+    return;
+  const auto node = torch::autograd::get_current_node();
+  for (size_t i = 0; node && i < node->num_outputs(); ++i) {
+    const auto& leaf = node->next_edge(i).function;
+    if (!leaf || leaf->num_outputs() != 0 ||
+        !node->task_should_compute_output(i))
+      continue;
+    const auto on = leaf->stream();
+    TORCH_CHECK(!on || on->id() != 0, what, ": a backward pass cannot be "
+                "captured while an eager graph of the same leaves lives: "
+                "delete its outputs first");
+  }
 }
 
 // A matrix of the rows of x whose rows are contiguous.
@@ -109,8 +127,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Tensor r = res ? matrix(*res) : Tensor();
     auto [y, h, rstd] = rms_norm_fwd(m, w, some(r), eps);
     ctx->save_for_backward({m, r, w, rstd});
-    if (!res) return {y.view(x.sizes())};
-    return {y.view(x.sizes()), h.view(x.sizes())};
+    // not views, which could not be changed in place
+    if (!res) return {at::_unsafe_view(y, x.sizes())};
+    return {at::_unsafe_view(y, x.sizes()), at::_unsafe_view(h, x.sizes())};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("rms_norm");

@@ -100,6 +100,12 @@ void dispatch(at::ScalarType t, const char* what, F f) {
   }
 }
 
+// A launch has fewer than 2^32 threads.
+static inline void check_grid(long blocks, long threads, const char* what) {
+  TORCH_CHECK(blocks * threads < (1l << 32), what,
+              ": more elements than a launch has threads for");
+}
+
 static inline hipStream_t stream() {
   return c10::hip::getCurrentHIPStream().stream();
 }

@@ -725,3 +725,272 @@ def test_refusals_on_the_gpu():
                            rand(4, 8).double())
     with pytest.raises(RuntimeError, match='float32'):
         functions.dropout(rand(4).double(), key_of(1, 2))
+
+
+# ---- what else a program does with them ------------------------------------
+
+def test_outputs_changed_in_place():
+    W, w = rand(20, 64).requires_grad_(), rand(64, seed=1).requires_grad_()
+    x = rand(2, 3, 64, seed=2).requires_grad_()
+    ids = torch.arange(6, device=DEV).view(2, 3)
+    ld = torch.tensor([-0.1], device=DEV)
+
+    def outputs():
+        q = x.view(2, 3, 1, 64)
+        return [functions.embed_id(ids, W), functions.rms_norm(x, w),
+                functions.dropout(x, key_of(1, 2)),
+                *functions.rms_norm(x, w, residual=x),
+                *functions.linear_attention(q, q, q, ld)]
+
+    for i in range(len(outputs())):
+        y = outputs()[i]
+        y *= 3
+        z = outputs()[i] * 3
+        assert torch.equal(y.detach(), z.detach())
+        for a, b in zip(*(torch.autograd.grad(o.sum(), (W, w, x),
+                                              allow_unused=True)
+                          for o in (y, z))):
+            assert (a is None) == (b is None)
+            assert a is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_operators_under_checkpoint(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    w = rand(64, seed=1).requires_grad_()
+    x = rand(2, 40, 64, seed=2).requires_grad_()
+    ld, key = torch.tensor([-0.1, -0.2], device=DEV), key_of(1, 2)
+
+    def layer(x):
+        y, h = functions.rms_norm(x, w, residual=x)
+        q = y.view(2, 40, 2, 32)
+        o, _ = functions.linear_attention(q, q, q, ld)
+        return functions.dropout(o.flatten(2) + h, key)
+
+    want = torch.autograd.grad(layer(x).sum(), (x, w))
+    for p in (x, w):
+        p.grad = None
+    checkpoint(layer, x, use_reentrant=reentrant).sum().backward()
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+def test_operators_in_inference_mode():
+    with torch.inference_mode():
+        W, w = rand(20, 64), rand(64, seed=1)
+        state = torch.zeros(6, 1, 64, 64, device=DEV)
+        ids = torch.arange(6, device=DEV)
+        x = functions.dropout(functions.embed_id(ids, W), key_of(1, 2))
+        y, h = functions.rms_norm(x, w, residual=x)
+        q = y.view(6, 1, 64)
+        ld = torch.tensor([-0.1], device=DEV)
+        o = ops.linear_attention_step(q, q, q, state, ld)
+        p, s = functions.linear_attention(q[:, None], q[:, None], q[:, None],
+                                          ld)
+        assert torch.allclose(o, p[:, 0], rtol=1e-5, atol=1e-5)
+        assert torch.allclose(s, state, rtol=1e-5, atol=1e-5)
+        ops.dropout_next_key(key_of(1, 2))
+
+
+def test_two_graphs_at_once():
+    """Neither shares its workspaces with the other one."""
+    ld = torch.tensor([-0.01], device=DEV)
+    inputs = [(torch.randint(0, 3000, (20000,), device=DEV),
+               rand(20000, 64, seed=i), rand(1, 4096, 1, 64, seed=i))
+              for i in range(2)]
+
+    W0 = rand(3000, 64)
+
+    def work(ids, gy, q):
+        W, q = W0.detach().requires_grad_(), q.detach().requires_grad_()
+        dW, = torch.autograd.grad(functions.embed_id(ids, W), W, gy)
+        o, _ = functions.linear_attention(q, q, q, ld)
+        dq, = torch.autograd.grad(o, q, torch.ones_like(o))
+        return [dW, o.detach(), dq]
+
+    want = [work(*x) for x in inputs]
+    graphs, got = [], []
+    for x in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(work(*x))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for outs in got:
+            for o in outs:
+                o.fill_(-1)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for p, q in zip(a, b):
+                assert torch.equal(p, q)
+
+
+def test_a_capture_beside_an_eager_graph_is_refused():
+    W = rand(50, 64).requires_grad_()
+    ids = torch.arange(9, device=DEV)
+    gy = rand(9, 64)
+    eager = functions.embed_id(ids, W)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='eager graph'):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(functions.embed_id(ids, W), W, gy)
+    # a forward pass alone can be captured, and all of it without the other
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = functions.embed_id(ids, W).detach()
+    graph.replay()
+    assert torch.equal(y, eager.detach())
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dW, = torch.autograd.grad(functions.embed_id(ids, W), W, gy)
+    graph.replay()
+    assert torch.equal(dW[:9], gy) and not dW[9:].any()
+
+
+def test_dropout_from_any_address():
+    for t in TYPES:
+        x = rand(5001, t=t)
+        for first in (1, 2, 3, 8):
+            y = x[first:]
+            assert torch.equal(functions.dropout(y, key_of(3, 4)),
+                               functions.dropout(y.clone(), key_of(3, 4)))
+
+
+def test_linear_attention_of_views_of_lengths_and_decays():
+    x = rand(2, 40, 2, 16)
+    lengths = torch.tensor([40, 9, 7, 9], device=DEV)[::2]
+    ld = torch.tensor([-0.1, 0.0, -0.3], device=DEV)[::2]
+    a = functions.linear_attention(x, x, x, ld, lengths=lengths)
+    b = functions.linear_attention(x, x, x, ld.clone(),
+                                   lengths=lengths.clone())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    # lengths outside of the batch's
+    a = functions.linear_attention(x, x, x, ld, lengths=torch.tensor(
+        [99, -5], device=DEV, dtype=torch.int32))
+    b = functions.linear_attention(x, x, x, ld, lengths=torch.tensor(
+        [40, 0], device=DEV))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_too_many_for_a_launch_is_refused():
+    ld = torch.zeros(1, device=DEV)
+    x = torch.zeros(2 ** 21, 1, 1, 1, device=DEV)
+    with pytest.raises(RuntimeError, match='2.21'):
+        functions.linear_attention(x, x, x, ld)
+    x = torch.zeros(2 ** 24, 1, 1, device=DEV)
+    with pytest.raises(RuntimeError, match='threads'):
+        ops.linear_attention_step(x, x, x, x[..., None].contiguous(), ld)
+    # rows of 256 elements have 64 lanes each
+    ids = torch.zeros(2 ** 26, device=DEV, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match='threads'):
+        functions.embed_id(ids, torch.zeros(1, 256, device=DEV))
+
+
+# ---- more than 2^31 elements -----------------------------------------------
+
+def test_embed_past_32_bits():
+    t, dim = torch.bfloat16, 520
+    vocab = 2 ** 22
+    W = torch.zeros(vocab, dim, device=DEV, dtype=t)
+    W[-8:] = rand(8, dim, t=t)
+    W.requires_grad_()
+    ids = torch.tensor([vocab - 1, 5, vocab - 8, vocab - 1], device=DEV)
+    gy = rand(4, dim, t=t, seed=1)
+    y = functions.embed_id(ids, W)
+    assert torch.equal(y.detach(), W.detach()[ids])
+    dW, = torch.autograd.grad(y, W, gy)
+    near(dW[-1], gy[0].double() + gy[3].double(),
+         4 * E * (gy[0].abs() + gy[3].abs()).double())
+    assert torch.equal(dW[-8], gy[2]) and torch.equal(dW[5], gy[1])
+    dW[-1] = dW[-8] = dW[5] = 0
+    assert not dW.view(torch.int64).any()
+    del W, dW, y
+    ids = torch.arange(vocab, device=DEV) % 50
+    ids[-1] = 50
+    W = rand(1100, dim, t=t).requires_grad_()
+    y = functions.embed_id(ids, W)
+    assert torch.equal(y.detach()[-60:], W.detach()[ids[-60:]])
+    gy = torch.zeros_like(y.detach())
+    gy[-60:] = rand(60, dim, t=t, seed=1)
+    dW, = torch.autograd.grad(y, W, gy)
+    assert torch.equal(dW[50], gy[-1])
+    want = torch.zeros(1100, dim, device=DEV, dtype=torch.float64)
+    want.index_add_(0, ids[-60:], gy[-60:].double())
+    # at most two of the terms of a sum are not zero
+    near(dW, want, 4 * E * torch.zeros_like(want).index_add_(
+        0, ids[-60:], gy[-60:].double().abs()))
+
+
+def test_rms_norm_past_32_bits():
+    t, rows, dim = torch.bfloat16, 2 ** 21 + 3, 1030
+    x = torch.empty(rows, dim, device=DEV, dtype=t)
+    x.copy_(rand(dim, t=t))
+    w = rand(dim, seed=1)
+    few = x[:7].clone().requires_grad_()
+    x.requires_grad_()
+    y = functions.rms_norm(x, w)
+    want = functions.rms_norm(few, w)
+    assert torch.equal(y.detach()[-7:], want.detach())
+    dx, = torch.autograd.grad(y, x, y.detach())
+    dw, = torch.autograd.grad(want, few, want.detach())
+    assert torch.equal(dx[-7:], dw)
+    del dx, y
+    with torch.no_grad():
+        q, scales = ops.rms_norm_fp8(x, w)
+        a, b = ops.rms_norm_fp8(few, w)
+    assert torch.equal(q[-7:].view(torch.int8), a.view(torch.int8))
+    assert torch.equal(scales[-7:], b)
+
+
+@pytest.mark.parametrize('strides', [
+    (2 ** 31 + 64, 128, 64, 1), (2 ** 31 + 65, 128, 64, 1),
+    (128, 2 ** 27 + 8, 64, 1)])
+def test_linear_attention_strides_past_32_bits(strides):
+    shape = (2, 17, 2, 64)
+    space = torch.empty(1 + sum(
+        (n - 1) * s for n, s in zip(shape, strides)), device=DEV,
+        dtype=torch.bfloat16)
+    q = space.as_strided(shape, strides)
+    q.copy_(rand(*shape, t=torch.bfloat16))
+    ld = torch.tensor([-0.1, -0.2], device=DEV)
+    c = q.contiguous().requires_grad_()
+    q.requires_grad_()
+    go = rand(*shape, t=torch.bfloat16, seed=1)
+    for a, b in zip(*((lambda o, s, x: [o.detach(), s.detach()] + list(
+            torch.autograd.grad(o, x, go)))(
+                *functions.linear_attention(x, x, x, ld), x)
+            for x in (q, c))):
+        assert torch.equal(a.contiguous(), b)
+
+
+def test_linear_attention_output_past_32_bits():
+    b, length, d, few = 4100, 4100, 128, 300  # few enough, and one segment
+    x = torch.zeros(b, length, 1, d, device=DEV, dtype=torch.bfloat16)
+    x[-few:] = rand(few, length, 1, d, t=torch.bfloat16)
+    ld = torch.tensor([-0.02], device=DEV)
+    c = x[-few:].clone().requires_grad_()
+    x.requires_grad_()
+    o, s = functions.linear_attention(x, x, x, ld)
+    p, r = functions.linear_attention(c, c, c, ld)
+    assert torch.equal(o.detach()[-few:], p.detach())
+    assert torch.equal(s.detach()[-few:], r.detach())
+    g, = torch.autograd.grad(o, x, o.detach())
+    h, = torch.autograd.grad(p, c, p.detach())
+    assert torch.equal(g[-few:], h)
+
+
+def test_step_of_states_past_32_bits():
+    b, d, few = 2 ** 17 + 3, 128, 5
+    q = rand(b, 1, d)
+    state = torch.zeros(b, 1, d, d, device=DEV)
+    state[-few:] = rand(few, 1, d, d, seed=1)
+    last = state[-few:].clone()
+    ld = torch.tensor([-0.02], device=DEV)
+    o = ops.linear_attention_step(q, q, q, state, ld)
+    p = ops.linear_attention_step(q[-few:], q[-few:], q[-few:], last, ld)
+    assert torch.equal(o[-few:], p) and torch.equal(state[-few:], last)
