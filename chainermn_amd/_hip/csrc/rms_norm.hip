@@ -12,8 +12,9 @@
 // is used; the backward pass adds x and the residual again, since the rounded
 // sum would leave its rounding in dw.  Sums and rstd are fp32.
 //
-// A row belongs to `tpr` threads, a wave or several, of 16 elements each: a
-// wave has a row of 1024, and no barrier.  32768 x 1024 in bf16 with a
+// A row belongs to `tpr` threads, 2^n of them, of 16 elements each: a wave has
+// a row of 1024 or several shorter ones, and no barrier.  (524288 rows of 64
+// in bf16, both passes: 81 us; with a wave for each row, 360 us.)  32768 x 1024 in bf16 with a
 // residual: forward 50 us, 5.3 TB/s, backward 65 us, 5.2 TB/s, and 5 us for
 // the last sum of dw.  e4m3 with groups of 128 of 16384 x 4096: 108 us, 4.3
 // TB/s; 64 x 1024: 6 us, a launch.
@@ -36,6 +37,10 @@ using Part = float[kHeld<T>][kWidth<T>];
 // for each wave of the workgroup and is written again by the next call, so
 // that calls alternate between two of them.
 __device__ __forceinline__ float row_sum(float v, int tpr, float* lds) {
+  if (tpr < 64) {
+    for (int off = tpr >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+  }
   v = wave_sum(v);
   if (tpr > 64) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -48,8 +53,7 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* lds) {
 }
 
 __device__ __forceinline__ float row_max(float v, int tpr, float* lds) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
+  for (int off = (tpr < 64 ? tpr : 64) >> 1; off > 0; off >>= 1)
     v = fmaxf(v, __shfl_xor(v, off, 64));
   if (tpr > 64) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -133,7 +137,7 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(
   for (long r0 = blockIdx.x * (long)per; r0 < rows;
        r0 += gridDim.x * (long)per, turn ^= 1) {
     long row = r0 + threadIdx.x / tpr;
-    const bool on = row < rows;  // whole waves, and all of them at barriers
+    const bool on = row < rows;  // the others are at barriers and shuffles
     if (!on) row = rows - 1;
     Part<T> h;
     const float rstd = read_row<T>(
@@ -190,7 +194,7 @@ __device__ __forceinline__ void store_e4m3(unsigned char* p, float scale,
 }
 
 // y in e4m3 with a scale for each row (group = 0) or each `group` columns,
-// 2^n of them that at most a wave holds: amax / 448.
+// 2^n of them that at most a row's threads and a wave hold: amax / 448.
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_fp8_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
@@ -318,8 +322,15 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(
       }
     }
   }
+  // rows of one wave, then those of several
+  for (int off = tpr; off < 64; off <<= 1)
+#pragma unroll
+    for (int k = 0; k < kHeld<T>; ++k)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) dw[k][i] += __shfl_xor(dw[k][i], off, 64);
+  const int unit = tpr < 64 ? 64 : tpr, units = blockDim.x / unit;
   float* out = part + blockIdx.x * (long)dim;
-  if (per == 1) {
+  if (units == 1) {
 #pragma unroll
     for (int k = 0; k < kHeld<T>; ++k) {
       const int c = (k * tpr + t) * VE;
@@ -327,8 +338,8 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(
     }
     return;
   }
-  for (int p = 0; p < per; ++p) {  // one row of threads after another
-    if (threadIdx.x / tpr == p) {
+  for (int p = 0; p < units; ++p) {  // one after another
+    if (threadIdx.x / unit == p && threadIdx.x % unit < tpr) {
 #pragma unroll
       for (int k = 0; k < kHeld<T>; ++k) {
         const int c = (k * tpr + t) * VE;
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(
 #pragma unroll
             for (int i = 0; i < VE; ++i) dw[k][i] += a[i];
           }
-          if (p + 1 == per) store<float, VE>(out + c, dw[k], dim - c);
+          if (p + 1 == units) store<float, VE>(out + c, dw[k], dim - c);
           else store<float, VE>(cols + c, dw[k], dim - c);
         }
       }
@@ -391,10 +402,9 @@ void check_weight(const torch::Tensor& w, const torch::Tensor& x) {
               "their type or float32, on their GPU");
 }
 
-Rows plan(long rows, long dim) {
+Rows plan(long rows, long dim, int tpr = 1) {
   TORCH_CHECK(dim >= 1 && dim <= kMaxDim, "rms_norm: rows of 1 to ", kMaxDim,
               " elements, not ", dim);
-  int tpr = 64;
   while (tpr * 16 < dim) tpr *= 2;
   return Rows{rows, (int)dim, tpr, tpr < 256 ? 256 : tpr};
 }
@@ -447,7 +457,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> rms_norm_fp8(
                              group <= 256 && dim % group == 0),
               "rms_norm_fp8: groups of 16, 32, 64, 128 or 256 columns that "
               "divide the row, not ", group);
-  const Rows r = plan(rows, dim);
+  // a group's columns have neighbouring threads
+  const Rows r = plan(rows, dim, group ? group * x.element_size() / 16 : 1);
   auto q = torch::empty({rows, dim},
                         x.options().dtype(at::kFloat8_e4m3fn));
   auto scales = torch::empty({rows, group ? dim / group : 1},

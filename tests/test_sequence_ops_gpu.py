@@ -994,3 +994,22 @@ def test_step_of_states_past_32_bits():
     o = ops.linear_attention_step(q, q, q, state, ld)
     p = ops.linear_attention_step(q[-few:], q[-few:], q[-few:], last, ld)
     assert torch.equal(o[-few:], p) and torch.equal(state[-few:], last)
+
+
+# ---- several rows of a norm in a wave ---------------------------------------
+
+@pytest.mark.parametrize('t', TYPES)
+@pytest.mark.parametrize('rows,dim', [
+    (1, 2), (70000, 16), (300, 17), (1000, 32), (4099, 48), (515, 128),
+    (129, 255), (100, 256), (65537, 1)])
+@pytest.mark.parametrize('residual', [False, True])
+def test_rms_norm_of_short_rows(t, rows, dim, residual):
+    test_rms_norm(t, rows, dim, residual)
+
+
+@pytest.mark.parametrize('t', TYPES)
+@pytest.mark.parametrize('rows,dim,group', [
+    (300, 16, 16), (300, 256, 256), (1000, 512, 256), (77, 64, None),
+    (77, 48, 16), (513, 33, None), (129, 128, 128), (70000, 5, None)])
+def test_rms_norm_fp8_of_short_rows(t, rows, dim, group):
+    test_rms_norm_fp8(t, rows, dim, group, rows % 2 == 1)
