@@ -212,10 +212,18 @@ __device__ __forceinline__ void to_frag(const float (&x)[8], frag (&f)[N]) {
   for (int n = 0; n < N; ++n) f[n] = w[n].f;
 }
 
-// The rows of a chunk between global memory and LDS: a thread's part.  WIDE
-// operands are aligned and read through a buffer resource that ends with the
-// last row, so that what lies behind it reads as zero without a branch.
-template <typename T, int D, int C, bool WIDE>
+// How rows lie in memory: they begin on 32 bits and are whole vectors of 16
+// bytes; or they begin and end on 32 bits; or neither.
+enum Edge { kVectors, kWords, kHalves };
+
+// The rows of a chunk between global memory and LDS: a thread's part, read
+// through a buffer resource that ends with the last row, so that what lies
+// behind it reads as zero without a branch, 16 bytes at once from any word.
+// Halves are read from the word they begin in and moved by half of it.
+// (4 x 2048 tokens, 8 heads of 57 and 79, trained in bf16: 124 us; by single
+// elements at the rows' ends, 146 us.  With the tests of words for vectors
+// too, 2 x 16384 tokens of heads of 128 take 2% longer.)
+template <typename T, int D, int C, Edge EDGE>
 struct Rows {
   static constexpr int VE = 16 / sizeof(T);
   static constexpr int kThreads = D * 4;
@@ -225,17 +233,18 @@ struct Rows {
     vec<T, VE> v[N];
     vec<unsigned, 4> u[N];
   };
+  unsigned more[EDGE == kHalves ? N : 1], shift[EDGE == kHalves ? N : 1];
 
-  // rows at or behind `n` and columns at or behind `cols` are zero
+  // rows at or behind `n` and vectors at or behind `cols` are zero
   __device__ __forceinline__ void read(const T* p, long stride, int n,
                                        int cols) {
     const int row = threadIdx.x / (D / VE);
     const int col = threadIdx.x % (D / VE) * VE;
-    if constexpr (WIDE) {
-      const int pitch = int(stride * sizeof(T));
-      const int rows = n < C ? n : C;
-      const auto rsrc = buffer(p, (rows - 1) * pitch +
-                                      cols * (int)sizeof(T));
+    const int pitch = int(stride * sizeof(T));
+    const int rows = n < C ? n : C;
+    const int bytes = (rows - 1) * pitch + cols * (int)sizeof(T);
+    if constexpr (EDGE != kHalves) {
+      const auto rsrc = buffer(p, bytes);
 #pragma unroll
       for (int i = 0; i < N; ++i)
         u[i] = __builtin_amdgcn_raw_buffer_load_b128(
@@ -243,39 +252,64 @@ struct Rows {
                                    col * (int)sizeof(T)
                              : kBehind, 0, 0);
     } else {
+      const int half = int(reinterpret_cast<uintptr_t>(p) & 2);
+      const auto rsrc = buffer((const char*)p - half, (bytes + half + 3) & ~3);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const T* src = p + (row + i * kStep) * stride + col;
-        const int left = row + i * kStep < n ? cols - col : 0;
-        if (left >= VE) {
-          v[i] = *reinterpret_cast<const typename anywhere<T, VE>::type*>(
-              src);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) v[i][e] = e < left ? src[e] : T(0.f);
-        }
+        const int at = half + (row + i * kStep) * pitch +
+                       col * (int)sizeof(T);
+        const int word =
+            col < cols && row + i * kStep < rows ? at & ~3 : kBehind;
+        u[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, word, 0, 0);
+        more[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, word, 16, 0);
+        shift[i] = (at & 2) * 8;
       }
     }
   }
 
+  // What was read of the columns before `cols`, and zero.
+  __device__ __forceinline__ vec<unsigned, 4> words(int i, int cols) const {
+    vec<unsigned, 4> w = u[i];
+    if constexpr (EDGE == kHalves) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        w[d] = __builtin_amdgcn_alignbit(d < 3 ? w[d < 3 ? d + 1 : 3] : more[i],
+                                         w[d], shift[i]);
+    }
+    if (EDGE != kVectors && cols % VE) {
+      const int col = threadIdx.x % (D / VE) * VE;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int left = cols - col - d * VE / 4;
+        w[d] = left >= VE / 4 ? w[d] : left > 0 ? w[d] & 0xffff : 0;
+      }
+    }
+    return w;
+  }
+
   // planes of terms, each C * PITCH
   template <int PITCH, bool LANE_ORDER>
-  __device__ __forceinline__ void write(short* tile) const {
+  __device__ __forceinline__ void write(short* tile, int cols) const {
     constexpr int NT = kTerms<T>;
     const int row = threadIdx.x / (D / VE);
     const int col = threadIdx.x % (D / VE) * VE;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       short* dst = tile + (row + i * kStep) * PITCH;
+      union {
+        vec<unsigned, 4> u;
+        vec<T, VE> v;
+      } x;
+      x.u = words(i, cols);
       unsigned w[NT][VE / 2];
 #pragma unroll
       for (int e = 0; e < VE; e += 2) {
         if constexpr (NT == 1) {
-          w[0][e / 2] = u[i][e / 2];
+          w[0][e / 2] = x.u[e / 2];
         } else {
           unsigned a[NT], b[NT];
-          cut<NT>(float(v[i][e]), a);
-          cut<NT>(float(v[i][e + 1]), b);
+          cut<NT>(float(x.v[e]), a);
+          cut<NT>(float(x.v[e + 1]), b);
 #pragma unroll
           for (int n = 0; n < NT; ++n) w[n][e / 2] = pair(a[n], b[n]);
         }
@@ -334,7 +368,7 @@ constexpr int kWavesOfUnit = kTerms<T> < 3 ? 4 : D == 64 ? 3 : 2;
 // A workgroup takes a segment of a sequence and head for a role; a wave
 // keeps 16 columns of the state.  OUT = false computes the state of the
 // segment alone.
-template <typename T, int D, bool WIDE, bool OUT>
+template <typename T, int D, Edge EDGE, bool OUT>
 __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
     Problem pr) {
   using L = Lds<T, D>;
@@ -393,7 +427,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
 
   // chunks on their way to LDS, in registers
   constexpr int kAhead = OUT ? 1 : 2;
-  Rows<T, D, C, WIDE> kr[kAhead], vr[kAhead], qr[OUT ? kAhead : 1];
+  Rows<T, D, C, EDGE> kr[kAhead], vr[kAhead], qr[OUT ? kAhead : 1];
   auto fetch = [&](int step, auto slot) {
     if (step >= chunks) return;
     constexpr int x = decltype(slot)::value;
@@ -491,9 +525,9 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
       else if (threadIdx.x < 2 * C)
         seen[i] = ro.inter * power(log2, d > 0 ? d : 0);
     }
-    kr[x].template write<L::kPitch, false>(kt);
-    vr[x].template write<L::kPitch, false>(vt);
-    if constexpr (OUT) qr[x].template write<L::kPitchQ, true>(qt);
+    kr[x].template write<L::kPitch, false>(kt, dk);
+    vr[x].template write<L::kPitch, false>(vt, dv);
+    if constexpr (OUT) qr[x].template write<L::kPitchQ, true>(qt, dk);
     fetch(step + kAhead, slot);
     __syncthreads();
 
@@ -596,7 +630,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
 
     if constexpr (OUT) {
       const int j = col0 + 4 * g;
-      if constexpr (WIDE) {  // dv is a multiple of 4
+      if constexpr (EDGE != kHalves) {
         const int pitch = int(ostride * sizeof(T));
         const auto rsrc = buffer(op + c * C * ostride,
                                  (n - 1) * pitch + dv * (int)sizeof(T));
@@ -604,15 +638,25 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
         for (int it = 0; it < 2; ++it) {
           const int at = j < dv ? (it * 16 + l) * pitch + j * (int)sizeof(T)
                                 : kBehind;
-          vec<T, 4> r;
+          union {
+            vec<T, 4> v;
+            vec<unsigned, sizeof(T)> u;
+          } r;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = T(o[it][e]);
-          if constexpr (sizeof(T) == 2)
-            __builtin_amdgcn_raw_buffer_store_b64(
-                __builtin_bit_cast(vec<unsigned, 2>, r), rsrc, at, 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b128(
-                __builtin_bit_cast(vec<unsigned, 4>, r), rsrc, at, 0, 0);
+          for (int e = 0; e < 4; ++e) r.v[e] = T(o[it][e]);
+          if (EDGE == kVectors || dv % 4 == 0) {
+            if constexpr (sizeof(T) == 2)
+              __builtin_amdgcn_raw_buffer_store_b64(r.u, rsrc, at, 0, 0);
+            else
+              __builtin_amdgcn_raw_buffer_store_b128(r.u, rsrc, at, 0, 0);
+          } else {  // the last words of a row are the next one's first
+#pragma unroll
+            for (int w = 0; w < (int)sizeof(T); ++w)
+              __builtin_amdgcn_raw_buffer_store_b32(
+                  r.u[w], rsrc,
+                  j + w * 4 / (int)sizeof(T) < dv ? at + 4 * w : kBehind, 0,
+                  0);
+          }
         }
       } else {
 #pragma unroll
@@ -792,18 +836,21 @@ torch::Tensor rows_of(const torch::Tensor& x) {
   return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous();
 }
 
-// Whether rows can be read by 16 bytes through a buffer resource: aligned,
-// not on top of each other, and a chunk of them (and of the output) within
-// 2^30 bytes.
-bool is_wide(const torch::Tensor& x) {
-  const int ve = 16 / (int)x.element_size();
-  bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
-            x.size(-1) % ve == 0;
+// And with tokens that are not on top of each other, nor so far apart that a
+// chunk of them exceeds a buffer resource.
+torch::Tensor tokens_of(const torch::Tensor& x) {
+  const long t = x.stride(1);
+  return x.size(1) == 1 || (t >= x.size(3) && t < (1l << 24))
+             ? rows_of(x) : x.contiguous();
+}
+
+Edge edge_of(const torch::Tensor& x) {
+  const int size = (int)x.element_size();
+  bool words = reinterpret_cast<uintptr_t>(x.data_ptr()) % 4 == 0 &&
+               x.size(-1) * size % 4 == 0;
   for (int i = 0; i + 1 < x.dim(); ++i)
-    ok = ok && (x.size(i) == 1 || x.stride(i) % ve == 0);
-  return ok && x.size(2) * x.size(3) < (1l << 21) &&
-         (x.size(1) == 1 || (x.stride(1) >= x.size(-1) &&
-                             x.stride(1) < (1l << 21)));
+    words = words && (x.size(i) == 1 || x.stride(i) * size % 4 == 0);
+  return !words ? kHalves : x.size(-1) * size % 16 ? kWords : kVectors;
 }
 
 Operand operand(const torch::Tensor& x) {
@@ -833,19 +880,19 @@ struct Cut {
   }
 };
 
-template <typename T, int D, bool WIDE>
+template <typename T, int D, Edge EDGE>
 void run_chunks(const Problem& pr, bool state) {
   const long problems = (long)pr.batch * pr.heads * pr.segments;
   const dim3 grid((problems + 7) / 8 * 8 * pr.roles);
   if (state) {
-    chunk_kernel<T, D, WIDE, false>
+    chunk_kernel<T, D, EDGE, false>
         <<<grid, dim3(D * 4), Lds<T, D>::kState * 2, stream()>>>(pr);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     join_kernel<<<dim3(D * D / (kThreads * 4), pr.batch * pr.heads),
                   dim3(kThreads), 0, stream()>>>(pr, D * D);
   } else {
     constexpr int lds = Lds<T, D>::kAll * 2;
-    auto kernel = chunk_kernel<T, D, WIDE, true>;
+    auto kernel = chunk_kernel<T, D, EDGE, true>;
     // above 64 KB a workgroup has to ask
     if (lds > 65536)
       C10_HIP_CHECK(hipFuncSetAttribute(
@@ -858,14 +905,19 @@ void run_chunks(const Problem& pr, bool state) {
 
 // The states of the first role's segments where `state`, and otherwise the
 // outputs of all roles.
-void run_roles(const Problem& pr, const Cut& cut, bool wide, at::ScalarType t,
-               bool state) {
+void run_roles(const Problem& pr, const Cut& cut, Edge edge,
+               at::ScalarType t, bool state) {
   dispatch(t, "linear_attention", [&](auto x) {
     using T = decltype(x);
-    if (cut.d == 64 && wide) run_chunks<T, 64, true>(pr, state);
-    else if (cut.d == 64) run_chunks<T, 64, false>(pr, state);
-    else if (wide) run_chunks<T, 128, true>(pr, state);
-    else run_chunks<T, 128, false>(pr, state);
+    auto go = [&](auto e) {
+      if (cut.d == 64) run_chunks<T, 64, decltype(e)::value>(pr, state);
+      else run_chunks<T, 128, decltype(e)::value>(pr, state);
+    };
+    if constexpr (sizeof(T) == 2)
+      if (edge == kHalves)
+        return go(std::integral_constant<Edge, kHalves>());
+    if (edge == kVectors) go(std::integral_constant<Edge, kVectors>());
+    else go(std::integral_constant<Edge, kWords>());
   });
 }
 
@@ -876,6 +928,8 @@ Problem problem(const torch::Tensor& q, const torch::Tensor& log_decay,
   TORCH_CHECK(q.size(1) < (1l << 30) && q.size(0) * q.size(2) < (1l << 21),
               "linear_attention: fewer than 2^30 tokens of a sequence and "
               "2^21 sequences times heads");
+  TORCH_CHECK(q.size(2) < (1l << 17), "linear_attention: fewer than 2^17 "
+              "heads");
   pr.batch = (int)q.size(0);
   pr.length = (int)q.size(1);
   pr.heads = (int)q.size(2);
@@ -914,9 +968,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
   const c10::DeviceGuard guard(q.device());
   const long b = q.size(0), h = q.size(2), dk = q.size(3), dv = v.size(3);
   if (first) check_state(*first, q, b, h, dk, dv);
-  q = rows_of(q);
-  k = rows_of(k);
-  v = rows_of(v);
+  q = tokens_of(q);
+  k = tokens_of(k);
+  v = tokens_of(v);
   const auto floats = q.options().dtype(at::kFloat);
   auto o = torch::empty({b, q.size(1), h, dv}, q.options());
   auto last = torch::empty({b, h, dk, dv}, floats);
@@ -937,9 +991,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
   r.dv = (int)dv;
   r.intra = r.inter = (float)scale;
   r.gain = 1.f;
-  const bool wide = is_wide(q) && is_wide(k) && is_wide(v);
-  if (cut.segments > 1) run_roles(pr, cut, wide, q.scalar_type(), true);
-  run_roles(pr, cut, wide, q.scalar_type(), false);
+  const Edge edge = std::max({edge_of(q), edge_of(k), edge_of(v)});
+  if (cut.segments > 1) run_roles(pr, cut, edge, q.scalar_type(), true);
+  run_roles(pr, cut, edge, q.scalar_type(), false);
   return {o, last, states};
 }
 
@@ -964,10 +1018,10 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   const long b = q.size(0), h = q.size(2), dk = q.size(3), dv = v.size(3);
   if (first) check_state(*first, q, b, h, dk, dv);
   if (glast) check_state(*glast, q, b, h, dk, dv);
-  q = rows_of(q);
-  k = rows_of(k);
-  v = rows_of(v);
-  go = rows_of(go);
+  q = tokens_of(q);
+  k = tokens_of(k);
+  v = tokens_of(v);
+  go = tokens_of(go);
   const auto floats = q.options().dtype(at::kFloat);
   auto gq = torch::empty(q.sizes(), q.options());
   auto gk = torch::empty(k.sizes(), k.options());
@@ -981,7 +1035,8 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
               states.scalar_type() == at::kFloat,
               "linear_attention: states of another call");
   auto gstates = torch::empty({cut.states(q)}, floats);
-  const bool wide = is_wide(q) && is_wide(k) && is_wide(v) && is_wide(go);
+  const Edge edge =
+      std::max({edge_of(q), edge_of(k), edge_of(v), edge_of(go)});
   const float c = (float)scale;
   Problem pr = problem(q, log_decay, lengths, cut);
   Role e{};  // dv = k G
@@ -1021,13 +1076,13 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   if (cut.segments > 1 && backwards) {
     pr.roles = 1;
     pr.role[0] = e;
-    run_roles(pr, cut, wide, q.scalar_type(), true);
+    run_roles(pr, cut, edge, q.scalar_type(), true);
   }
   pr.roles = 0;
   if (need_v || need_first) pr.role[pr.roles++] = e;
   if (need_k) pr.role[pr.roles++] = f;
   if (need_q) pr.role[pr.roles++] = a;
-  if (pr.roles) run_roles(pr, cut, wide, q.scalar_type(), false);
+  if (pr.roles) run_roles(pr, cut, edge, q.scalar_type(), false);
   return {gq, gk, gv, gfirst};
 }
 

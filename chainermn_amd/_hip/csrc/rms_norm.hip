@@ -14,10 +14,11 @@
 //
 // A row belongs to `tpr` threads, 2^n of them, of 16 elements each: a wave has
 // a row of 1024 or several shorter ones, and no barrier.  (524288 rows of 64
-// in bf16, both passes: 81 us; with a wave for each row, 360 us.)  32768 x 1024 in bf16 with a
-// residual: forward 50 us, 5.3 TB/s, backward 65 us, 5.2 TB/s, and 5 us for
-// the last sum of dw.  e4m3 with groups of 128 of 16384 x 4096: 108 us, 4.3
-// TB/s; 64 x 1024: 6 us, a launch.
+// in bf16, both passes: 81 us; with a wave for each row, 360 us.)
+//
+// 32768 x 1024 in bf16 with a residual: forward 50 us, 5.3 TB/s, backward 65
+// us, 5.2 TB/s, and 5 us for the last sum of dw.  e4m3 with groups of 128 of
+// 16384 x 4096: 108 us, 4.3 TB/s; 64 x 1024: 6 us, a launch.
 
 #include "seq_common.h"
 

@@ -1013,3 +1013,59 @@ def test_rms_norm_of_short_rows(t, rows, dim, residual):
     (77, 48, 16), (513, 33, None), (129, 128, 128), (70000, 5, None)])
 def test_rms_norm_fp8_of_short_rows(t, rows, dim, group):
     test_rms_norm_fp8(t, rows, dim, group, rows % 2 == 1)
+
+
+# ---- rows of attention that are no whole vectors -----------------------------
+
+@pytest.mark.parametrize('t', TYPES)
+@pytest.mark.parametrize('b,length,h,dk,dv', [
+    (2, 70, 3, 102, 96), (2, 33, 2, 2, 126), (1, 65, 5, 31, 117),
+    (3, 40, 1, 82, 20), (2, 37, 4, 7, 5), (1, 64, 1, 127, 1),
+    (2, 290, 1, 58, 63)])
+@pytest.mark.parametrize('ragged', [False, True])
+def test_linear_attention_of_odd_heads(t, b, length, h, dk, dv, ragged):
+    attention_case(t, b, length, h, dk, dv, ragged, state=not ragged)
+
+
+@pytest.mark.parametrize('t', TYPES)
+def test_linear_attention_of_odd_strides(t):
+    for first, behind in ((1, 0), (1, 1), (2, 1), (0, 3), (3, 1)):
+        for d in (64, 33, 30):
+            attention_case(
+                t, 2, 70, 2, d, d, True, False,
+                make=lambda x: torch.nn.functional.pad(
+                    x, (first, behind))[..., first:first + x.shape[-1]])
+
+
+@pytest.mark.parametrize('t', TYPES)
+@pytest.mark.parametrize('d', [1, 7, 31, 63, 66, 127])
+def test_linear_attention_of_odd_heads_reads_nothing_behind_the_end(t, d):
+    """The first word behind a row can hold the next row's first element."""
+    ld = torch.tensor([-0.2], device=DEV)
+    q, k, v = (rand(3, 70, 1, d, t=t, seed=i) for i in range(3))
+    lengths = torch.tensor([37, 0, 64], device=DEV)
+    clean, dirty = [], []
+    for x in (q, k, v):
+        x, y = x.clone(), x.clone()
+        for b in range(3):
+            x[b, lengths[b]:] = 0
+            y[b, lengths[b]:] = float('nan')
+        clean.append(x.requires_grad_())
+        dirty.append(y.requires_grad_())
+    go = rand(3, 70, 1, d, t=t, seed=5)
+    for a, b in zip(*(
+            (lambda o, s, xs: [o.detach(), s.detach()] + list(
+                torch.autograd.grad((o, s), xs, (go, torch.ones_like(s)))))(
+                *functions.linear_attention(*xs, ld, lengths=lengths), xs)
+            for xs in (clean, dirty))):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_linear_attention_of_tokens_on_top_of_each_other():
+    x = rand(2, 200, 2, 16, seed=1)
+    for strides in ((32, 0, 16, 1), (6400, 16, 8, 1), (0, 32, 16, 1)):
+        y = x.as_strided((2, 90, 2, 16), strides)
+        ld = torch.tensor([-0.2, -0.1], device=DEV)
+        a = functions.linear_attention(y, y, y, ld)
+        b = functions.linear_attention(*[y.contiguous()] * 3, ld)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
