@@ -440,6 +440,9 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
 
   // the state: tile t has rows 16t + 4g + r of dk, column col0 + l of dv
   const int col0 = wave * 16;
+  // Waves behind the last column read and compute scores only.  (Heads of 82
+  // and 20, 8 x 2670 tokens, 10 heads, forward in bf16: 101 us -> 90 us.)
+  const bool busy = col0 < dv;
   acc4 s[KT];
   bool some = true;  // whether the state can be other than zero
   float* stored = ro.states + ((long)bh * pr.segments + seg) * (D * D);
@@ -562,7 +565,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
       }
 
       // q S, transposed: rows of dv, columns i
-      if (some) {
+      if (some && busy) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           float x[8];
@@ -588,6 +591,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
       }
       __syncthreads();  // the scores are whole
     }
+    if (!busy) return;
 
     if constexpr (OUT) {
       decay_state(less);
