@@ -1069,3 +1069,9 @@ def test_linear_attention_of_tokens_on_top_of_each_other():
         a = functions.linear_attention(y, y, y, ld)
         b = functions.linear_attention(*[y.contiguous()] * 3, ld)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_too_many_heads_are_refused():
+    x = torch.zeros(1, 1, 2 ** 17, 1, device=DEV)
+    with pytest.raises(RuntimeError, match='2.17'):
+        functions.linear_attention(x, x, x, torch.zeros(2 ** 17, device=DEV))
