@@ -4,8 +4,8 @@
 //   dW[v] = c * sum of gy[t] over id_t == v   (the whole table, zeros too)
 //
 // Both are bound by memory.  32768 tokens of 32000 x 1024 in fp32: the lookup
-// takes 39 us, 5 TB/s of what it has to move, and the gradient 83 us: 57 us
-// for embed_rows, 4.7 TB/s, 20 us for the order and 7 us for embed_join.
+// takes 39 us, 5 TB/s of what it has to move, and the gradient 80 us: 55 us
+// for embed_rows, 4.8 TB/s, 18 us for the order and 7 us for embed_join.
 // (With one sorting pass, in which every workgroup reads all ids, the order
 // alone took 50 us.)
 //
@@ -17,7 +17,9 @@
 //      then each of these buckets by the others.  A bucket's workgroup finds
 //      its place in the order from the counts of all of them, so none waits
 //      for another one.  Low bits, because the frequent words of a vocabulary
-//      sorted by frequency are neighbours.
+//      sorted by frequency are neighbours.  16 waves: the bucket of the most
+//      frequent word lasts longest.  (262144 tokens, 7% of them one word, both
+//      passes: 402 us; with 8 waves 429 us.)
 //   2. embed_rows: a wave sums 8 to 32 sorted tokens of some columns; rows
 //      that begin and end within its tokens are finished, the two at its
 //      ends leave partial sums.  So a frequent word costs no more than
@@ -31,8 +33,8 @@ namespace {
 using namespace seq;
 
 constexpr int kSplitThreads = 1024, kSplitWaves = kSplitThreads / 64;
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr int kMaxBins = 1024;    // ids of a workgroup of embed_sort
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kMaxBins = 512;     // ids of a workgroup of embed_sort
 constexpr int kMaxPieces = 1024;  // workgroups of embed_split
 constexpr int kJoinWaves = 8;
 
@@ -590,7 +592,7 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return dw;
   }
-  // 256 buckets, or as many as leave 1024 ids to each; above 2^19 ids a
+  // 256 buckets, or 512 where these have 512 ids and more; above 2^18 ids a
   // bucket is sorted in parts
   int bucket_bits = 0;
   while (bucket_bits < 8 && (1l << bucket_bits) < vocab) ++bucket_bits;
