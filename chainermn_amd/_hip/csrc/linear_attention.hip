@@ -863,18 +863,21 @@ Operand operand(const torch::Tensor& x) {
                  x.size(1) == 1 ? x.size(3) : x.stride(1), x.stride(2)};
 }
 
-// The lengths of segments: 4 chunks and more, as long as there are no more
-// than 2048 waves, eight on each CU; more of them cost more in joining states
-// than they gain.  (2 x 16384 tokens, 8 heads of 128, trained: 342 us, and 352
-// us with twice as many; 4 x 2048, 16 heads of 64: 160 us, and 174 us with
-// half.)  A call and its backward pass cut alike.
+// The lengths of segments: 2 chunks and more where there are 8 of them (546
+// tokens, 8 heads, forward: 21 us, with 4 and more 27 us; 256 tokens, 16 heads:
+// 20 us both in one segment and in four), as long as there are no more than
+// 2048 waves, eight on each CU; more of them cost more in joining states than
+// they gain.  (2 x 16384 tokens, 8 heads of 128, trained: 342 us, and 352 us
+// with twice as many; 4 x 2048, 16 heads of 64: 160 us, and 174 us with half.)
+// A call and its backward pass cut alike.
 struct Cut {
   int d, segments, per_segment;
   Cut(const torch::Tensor& q, const torch::Tensor& v) {
     d = q.size(3) <= 64 && v.size(3) <= 64 ? 64 : 128;
     const long alone = q.size(0) * q.size(2);
     const long chunks = (q.size(1) + kChunk - 1) / kChunk;
-    const long n = std::max(1l, std::min(32768 / d / alone, chunks / 4));
+    const long most = chunks >= 8 ? chunks / 2 : 1;
+    const long n = std::max(1l, std::min(32768 / d / alone, most));
     const long per = std::max(1l, (chunks + n - 1) / n);
     per_segment = int(per * kChunk);
     segments = std::max(1, int((chunks + per - 1) / per));
