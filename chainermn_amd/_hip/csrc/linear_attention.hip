@@ -213,8 +213,9 @@ __device__ __forceinline__ void to_frag(const float (&x)[8], frag (&f)[N]) {
 }
 
 // How rows lie in memory: they begin on 32 bits and are whole vectors of 16
-// bytes; or they begin and end on 32 bits; or neither.
-enum Edge { kVectors, kWords, kHalves };
+// bytes, more than half of D each, or one of them not more; or they begin and
+// end on 32 bits; or neither.
+enum Edge { kVectors, kShort, kWords, kHalves };
 
 // The rows of a chunk between global memory and LDS: a thread's part, read
 // through a buffer resource that ends with the last row, so that what lies
@@ -276,7 +277,7 @@ struct Rows {
         w[d] = __builtin_amdgcn_alignbit(d < 3 ? w[d < 3 ? d + 1 : 3] : more[i],
                                          w[d], shift[i]);
     }
-    if (EDGE != kVectors && cols % VE) {
+    if (EDGE > kShort && cols % VE) {
       const int col = threadIdx.x % (D / VE) * VE;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
@@ -443,13 +444,16 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
   // Waves behind the last column read and compute scores only.  (Heads of 82
   // and 20, 8 x 2670 tokens, 10 heads, forward in bf16: 101 us -> 90 us.)
   const bool busy = col0 < dv;
-  // And the products end with the half of D in which the last of dk lies, or
-  // the quarter: more tests cost whole heads more than they give.  (16 x 2048
-  // tokens, 8 heads of 64 and 128, trained in bf16: 315 us -> 271 us; 2 x 6010
-  // tokens, 11 heads of 31 and 117 in fp32: 433 us -> 350 us; 4129 tokens of
-  // 102 and 96, forward: 115 us -> 120 us.)
-  constexpr int kPart = EDGE == kVectors ? D / 2 : D / 4;
-  auto behind = [&](int row) { return row % kPart == 0 && row >= dk; };
+  // And the products end with the quarter of D in which the last of dk lies,
+  // or with its half.  (16 x 2048 tokens, 8 heads of 64 and 128, trained in
+  // bf16: 315 us, 284 us by quarters, 275 us by halves; 2 x 6010 tokens, 11
+  // heads of 31 and 117 in fp32: 433 us, 350 us by quarters, 371 us by halves;
+  // 4129 tokens of 102 and 96, forward: 115 us -> 120 us.  Whole heads have no
+  // such tests, which would cost them 1 to 2%.)
+  constexpr int kPart = EDGE == kShort ? D / 2 : D / 4;
+  auto behind = [&](int row) {
+    return EDGE != kVectors && row % kPart == 0 && row >= dk;
+  };
   acc4 s[KT];
   bool some = true;  // whether the state can be other than zero
   float* stored = ro.states + ((long)bh * pr.segments + seg) * (D * D);
@@ -658,7 +662,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
           } r;
 #pragma unroll
           for (int e = 0; e < 4; ++e) r.v[e] = T(o[it][e]);
-          if (EDGE == kVectors || dv % 4 == 0) {
+          if (EDGE <= kShort || dv % 4 == 0) {
             if constexpr (sizeof(T) == 2)
               __builtin_amdgcn_raw_buffer_store_b64(r.u, rsrc, at, 0, 0);
             else
@@ -897,6 +901,10 @@ struct Cut {
   }
 };
 
+Edge edge_of_heads(long dk, long dv, const Cut& cut) {
+  return std::min(dk, dv) <= cut.d / 2 ? kShort : kVectors;
+}
+
 template <typename T, int D, Edge EDGE>
 void run_chunks(const Problem& pr, bool state) {
   const long problems = (long)pr.batch * pr.heads * pr.segments;
@@ -934,6 +942,7 @@ void run_roles(const Problem& pr, const Cut& cut, Edge edge,
       if (edge == kHalves)
         return go(std::integral_constant<Edge, kHalves>());
     if (edge == kVectors) go(std::integral_constant<Edge, kVectors>());
+    else if (edge == kShort) go(std::integral_constant<Edge, kShort>());
     else go(std::integral_constant<Edge, kWords>());
   });
 }
@@ -1008,7 +1017,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_attention_fwd(
   r.dv = (int)dv;
   r.intra = r.inter = (float)scale;
   r.gain = 1.f;
-  const Edge edge = std::max({edge_of(q), edge_of(k), edge_of(v)});
+  const Edge edge = std::max({edge_of(q), edge_of(k), edge_of(v),
+                              edge_of_heads(dk, dv, cut)});
   if (cut.segments > 1) run_roles(pr, cut, edge, q.scalar_type(), true);
   run_roles(pr, cut, edge, q.scalar_type(), false);
   return {o, last, states};
@@ -1052,8 +1062,8 @@ linear_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
               states.scalar_type() == at::kFloat,
               "linear_attention: states of another call");
   auto gstates = torch::empty({cut.states(q)}, floats);
-  const Edge edge =
-      std::max({edge_of(q), edge_of(k), edge_of(v), edge_of(go)});
+  const Edge edge = std::max({edge_of(q), edge_of(k), edge_of(v), edge_of(go),
+                              edge_of_heads(dk, dv, cut)});
   const float c = (float)scale;
   Problem pr = problem(q, log_decay, lengths, cut);
   Role e{};  // dv = k G
