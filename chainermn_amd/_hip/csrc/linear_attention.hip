@@ -346,6 +346,36 @@ __device__ __forceinline__ float power(float log2, int n) {
   return __builtin_amdgcn_exp2f(log2 * n);
 }
 
+// What a state goes through in n tokens, s lam^n.  While lam^n is above a half
+// it is s + s (lam^n - 1): rounded to fp32, a lam^n near one would lose what a
+// long memory forgets, the same in each chunk.  Below, lam^n - 1 has lost lam^n
+// (at lam^n = 1e-7 all but one bit of it), and the plain product comes before
+// a sum with nothing.  Both change the state where it is: with a branch to one
+// or the other the compiler copied it behind the products into it, and of the
+// ways out of their loop its waits took the longer one for the shorter, so that
+// a copy came before the product's result.
+struct Decay {
+  float by = 0.f, far = 1.f;
+  __device__ __forceinline__ void set(float ld, int n) {
+    const float x = ld * n;
+    const bool near = x > -0.6931f;
+    by = near ? expm1f(x) : 0.f;
+    far = near ? 1.f : expf(x);
+  }
+  template <int N>
+  __device__ __forceinline__ void operator()(acc4 (&s)[N]) const {
+    if (far != 1.f) {
+#pragma unroll
+      for (int t = 0; t < N; ++t) s[t] *= far;
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        s[t][r] = __builtin_fmaf(s[t][r], by, s[t][r]);
+  }
+};
+
 // LDS of a workgroup, in elements of 16 bits.
 template <typename T, int D>
 struct Lds {
@@ -496,15 +526,12 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
       reinterpret_cast<unsigned*>(pt)[i] = 0;
   }
 
-  auto decay_state = [&](float by) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s[t][r] = __builtin_fmaf(s[t][r], by, s[t][r]);
-  };
+  Decay decay;
   if constexpr (!OUT) {
-    if (some) decay_state(expm1f(ld * live));
+    if (some) {
+      decay.set(ld, live);
+      decay(s);
+    }
   }
   // Three waves have a tile of scores each, (0, 0), (1, 1) and the one between
   // them, and the factors of its elements; zero where the mask is.
@@ -517,8 +544,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
     const int d = rev ? j - i : i - j;
     fade[r] = d >= 0 ? ro.intra * power(log2, d) : 0.f;
   }
-  int of_tables = 0;   // the n that tables and `less` are for
-  float less = 0.f;    // lam^n - 1, which keeps a decay near one exact
+  int of_tables = 0;  // the n that tables and `decay` are for
   auto chunk = [&](int step, auto slot) {
     constexpr int x = decltype(slot)::value;
     const int c = rev ? chunks - 1 - step : step;
@@ -532,7 +558,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
       if (i < C) gain[i] = ro.gain * power(log2, d > 0 ? d : 0);
     } else if (n != of_tables) {  // the first chunk, and one not full
       of_tables = n;
-      less = expm1f(ld * n);
+      decay.set(ld, n);
       const int i = threadIdx.x % C;
       const int d = rev ? n - 1 - i : i + 1, e = rev ? i + 1 : n - 1 - i;
       if (threadIdx.x < C) gain[i] = ro.gain * power(log2, e > 0 ? e : 0);
@@ -607,7 +633,7 @@ __global__ __launch_bounds__(D * 4, (kWavesOfUnit<T, D>)) void chunk_kernel(
     if (!busy) return;
 
     if constexpr (OUT) {
-      decay_state(less);
+      decay(s);
       some = true;
     }
 
@@ -726,9 +752,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Problem pr,
   const float ld = decay_of(pr, bh % pr.heads);
   float* p = ro.states + (long)bh * pr.segments * elements +
              (blockIdx.x * kThreads + threadIdx.x) * 4;
-  acc4 carry = {};
+  acc4 carry[1] = {};
   int of = -1;
-  float less = 0.f;
+  Decay decay;
   constexpr int U = 16;
   for (int i0 = 0; i0 < pr.segments; i0 += U) {
     acc4 own[U];
@@ -744,15 +770,15 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Problem pr,
       if (i < pr.segments) {
         // the entry's own state holds what came in; the exit's is not
         // computed, nor used
-        if (i > 0) *reinterpret_cast<acc4*>(p + (long)seg * elements) = carry;
+        if (i > 0)
+          *reinterpret_cast<acc4*>(p + (long)seg * elements) = carry[0];
         const long left = len - (long)seg * pr.per_segment;
         const int n = left < 0 ? 0
                       : left < pr.per_segment ? int(left) : pr.per_segment;
-        if (n != of) less = expm1f(ld * n);
+        if (n != of) decay.set(ld, n);
         of = n;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          carry[r] = __builtin_fmaf(carry[r], less, carry[r]) + own[u][r];
+        decay(carry);
+        carry[0] += own[u];
       }
     }
   }
