@@ -5,12 +5,17 @@ The state is a buffer of two integers, a seed and the number of calls so far:
 it moves with the model, is saved with it, and a restored model goes on with
 the same numbers.  It is counted up on the GPU, so a replayed graph draws new
 ones.  Ranks given their communicator draw from streams of their own, also
-after ``bcast_data`` has made their states equal."""
+after ``bcast_data`` has made their states equal.
+
+A call that is computed again in a backward pass has to drop what it dropped
+first: checkpoint it by ``functions.forget``.  Under ``torch.utils.checkpoint``,
+which does not know the state, it raises an error."""
 
 import torch
 import torch.nn as nn
 
 from chainermn_amd import functions, ops
+from chainermn_amd.functions.forget import dropout_key
 from chainermn_amd.ops._dropout import dropout_threshold
 
 
@@ -29,7 +34,8 @@ class FusedDropout(nn.Module):
     def forward(self, x):
         if not self.training or self.ratio == 0.0:
             return x
-        key = ops.dropout_next_key(self.rng_state, self.stream)
+        key = dropout_key(lambda: ops.dropout_next_key(self.rng_state,
+                                                       self.stream))
         return functions.dropout(x, key, ratio=self.ratio)
 
     def extra_repr(self):

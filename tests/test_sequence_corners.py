@@ -1,0 +1,149 @@
+"""Corners of the sequence-model links and models, on the CPU."""
+
+import pytest
+import torch
+import torch.nn as nn
+from torch.utils.checkpoint import checkpoint
+
+from chainermn_amd import functions, links
+
+
+# ---- dropout that is computed again ------------------------------------------
+
+def grads_of(make, run, x):
+    """The output, gradients and dropouts' states of a new module."""
+    torch.manual_seed(5)
+    module = make()
+    x = x.clone().requires_grad_()
+    y = run(module, x)
+    y.square().sum().backward()
+    return [y.detach(), x.grad] + [p.grad for p in module.parameters()] + [
+        b for name, b in module.named_buffers() if 'rng_state' in name]
+
+
+def same(got, want):
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert (a is None and b is None) or torch.equal(a, b)
+
+
+def layers():
+    return nn.ModuleList([nn.Linear(12, 12), links.FusedDropout(0.4),
+                          nn.Linear(12, 12)])
+
+
+def segment(module, x):
+    a, d, b = module
+    h = d(a(x)) * x  # the link twice, and its outputs are factors
+    return x + d(b(h)) * h
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_dropout_in_forgotten_segments(reentrant):
+    x = torch.randn(7, 12)
+
+    def plain(module, x):
+        return segment(module, segment(module, x))
+
+    def forgotten(module, x):
+        for _ in range(2):
+            x = functions.forget(lambda t: segment(module, t), x,
+                                 use_reentrant=reentrant)
+        return x
+
+    want = grads_of(layers, plain, x)
+    assert want[-1][1] == 4  # calls
+    same(grads_of(layers, forgotten, x), want)
+
+
+@pytest.mark.parametrize('outer', [False, True])
+@pytest.mark.parametrize('inner', [False, True])
+def test_dropout_in_nested_forgotten_segments(outer, inner):
+    x = torch.randn(7, 12)
+
+    def twice(module, x):
+        for _ in range(2):
+            x = functions.forget(lambda t: segment(module, t), x,
+                                 use_reentrant=inner)
+        return segment(module, x)
+
+    want = grads_of(layers, lambda m, x: segment(m, segment(m, segment(
+        m, x))), x)
+    same(grads_of(layers, lambda m, x: functions.forget(
+        lambda t: twice(m, t), x, use_reentrant=outer), x), want)
+
+
+def test_a_forgotten_segment_can_be_differentiated_twice_over():
+    torch.manual_seed(5)
+    module, x = layers(), torch.randn(7, 12, requires_grad=True)
+    y = functions.forget(lambda t: segment(module, t), x)
+    first, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    # a call in between has numbers of its own and takes none away
+    module[1](torch.ones(100))
+    again, = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(first, again) and module[1].rng_state[1] == 3
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_attention_rnn_with_dropout_forgotten(reentrant):
+    x = torch.randn(3, 9, 16)
+
+    def make():
+        return links.LinearAttentionRNN(16, 16, num_layers=2, n_heads=2,
+                                        dropout=0.3)
+
+    want = grads_of(make, lambda m, x: m(x)[0], x)
+    same(grads_of(make, lambda m, x: functions.forget(
+        lambda t: m(t)[0], x, use_reentrant=reentrant), x), want)
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_dropout_under_a_checkpoint_that_does_not_know_it(reentrant):
+    module, x = layers(), torch.randn(7, 12, requires_grad=True)
+
+    def run(x):
+        return checkpoint(lambda t: segment(module, t), x,
+                          use_reentrant=reentrant).sum()
+
+    loss = run(x)
+    with pytest.raises(RuntimeError, match='functions.forget'):
+        loss.backward()
+    # without a forgotten call around it, being within one does not help
+    loss = functions.forget(run, x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match='functions.forget'):
+        loss.backward()
+    module.eval()  # nothing is dropped, and nothing is refused
+    run(x).backward()
+    assert torch.isfinite(x.grad).all()
+
+
+def test_a_recomputation_that_drops_more_often():
+    d, x = links.FusedDropout(0.4), torch.randn(8, requires_grad=True)
+    calls = []
+
+    def growing(x):
+        calls.append(0)
+        for _ in calls:
+            x = d(x)
+        return x.square()
+
+    y = functions.forget(growing, x, use_reentrant=True)
+    with pytest.raises(RuntimeError, match='more often'):
+        y.sum().backward()
+    # and neither call leaves a recomputation open behind it
+    first, second = d(torch.ones(100)), d(torch.ones(100))
+    assert not torch.equal(first, second)
+
+
+def test_a_forgotten_segment_that_fails():
+    d, x = links.FusedDropout(0.4), torch.randn(8, requires_grad=True)
+
+    def broken(x):
+        d(x)
+        raise KeyError('broken')
+
+    with pytest.raises(KeyError):
+        functions.forget(broken, x)
+    y = functions.forget(lambda t: d(t) * t, x)
+    g, = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(g != 0, y != 0) and d.rng_state[1] == 2

@@ -6,11 +6,12 @@ known in 64 bits.
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
-    from chainermn_amd import functions
+    from chainermn_amd import functions, links
     DEV = torch.device('cuda:0')
 else:
     pytest.skip('needs ROCm GPU', allow_module_level=True)
@@ -77,3 +78,87 @@ def test_a_state_that_nothing_is_added_to_decays(t, length, rate):
     close(o.detach(), want * lam[1:, None, None], sums(dk), dk * least)
     want = torch.einsum('bthj,bhij->bthi', v.double(), gs.double())
     close(gk, want * lam[:-1].flip(0)[:, None, None], sums(dv), dv * least)
+
+
+# ---- dropout that is computed again ------------------------------------------
+
+def dropout_layers():
+    torch.manual_seed(5)
+    return torch.nn.ModuleList([
+        torch.nn.Linear(64, 64, bias=False), links.FusedDropout(0.4),
+        links.LinearAttentionRNN(64, 64, num_layers=2, n_heads=2,
+                                 dropout=0.3)]).to(DEV)
+
+
+def dropout_segment(module, x):
+    a, d, rnn = module
+    h = d(a(x)) * x
+    return x + d(rnn(h)[0]) * h
+
+
+def dropout_grads(module, y):
+    # of y.square().sum(); a captured sum over many blocks clears memory in a
+    # way that replays do not repeat
+    return torch.autograd.grad(y, list(module.parameters()), 2 * y.detach())
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_dropout_in_a_forgotten_segment(reentrant):
+    x = rand(3, 50, 64)
+    want_module, module = dropout_layers(), dropout_layers()
+    want = dropout_segment(want_module, x)
+    want_grads = dropout_grads(want_module, want)
+    for p in module.parameters():
+        p.grad = None
+    x.requires_grad_()
+    got = functions.forget(lambda t: dropout_segment(module, t), x,
+                           use_reentrant=reentrant)
+    got.backward(2 * got.detach())
+    assert torch.equal(got, want)
+    for p, w in zip(module.parameters(), want_grads):
+        assert torch.equal(p.grad, w)
+    assert module[1].rng_state.tolist() == want_module[1].rng_state.tolist()
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_dropout_under_a_checkpoint_that_does_not_know_it(reentrant):
+    module, x = dropout_layers(), rand(3, 50, 64).requires_grad_()
+    y = checkpoint(lambda t: dropout_segment(module, t), x,
+                   use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match='functions.forget'):
+        y.sum().backward()
+
+
+def test_a_forgotten_segment_in_a_graph():
+    """Each replay draws new numbers, and its recomputation the same ones."""
+    module, x = dropout_layers(), rand(3, 50, 64)
+
+    def work():
+        y = functions.forget(lambda t: dropout_segment(module, t), x,
+                             preserve_rng_state=False)
+        return [y.detach()] + list(dropout_grads(module, y))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    states = [b for n, b in module.named_buffers() if 'rng_state' in n]
+    start = [b.clone() for b in states]
+    replays = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        replays.append([g.clone() for g in got])
+    for b, s in zip(states, start):
+        b.copy_(s)
+    for one in replays:
+        y = dropout_segment(module, x)
+        want = [y.detach()] + list(dropout_grads(module, y))
+        for a, b in zip(one, want):
+            assert torch.equal(a, b)
+        del y, want
+    assert not torch.equal(replays[0][0], replays[1][0])
