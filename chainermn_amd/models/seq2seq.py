@@ -112,7 +112,7 @@ class Seq2Seq(nn.Module):
     def translate(self, xs, max_length, bos=0, lengths=None):
         """Greedy generation (the reference's ``translate``): the
         ``[batch, max_length]`` tokens that follow ``bos``."""
-        training = self.training
+        modes = [(m, m.training) for m in self.modules()]
         self.eval()
         try:
             state = self.encoder(xs, lengths)
@@ -124,7 +124,8 @@ class Seq2Seq(nn.Module):
                 y = logits.argmax(-1)
                 out.append(y)
         finally:
-            self.train(training)
+            for m, training in modes:  # parts of it may be frozen
+                m.training = training
         return torch.stack(out, 1) if out else xs.new_empty(
             (xs.shape[0], 0), dtype=torch.long)
 

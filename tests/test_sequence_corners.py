@@ -6,6 +6,7 @@ import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
 from chainermn_amd import functions, links
+from chainermn_amd.models.seq2seq import Seq2Seq
 
 
 # ---- dropout that is computed again ------------------------------------------
@@ -147,3 +148,17 @@ def test_a_forgotten_segment_that_fails():
     y = functions.forget(lambda t: d(t) * t, x)
     g, = torch.autograd.grad(y.sum(), x)
     assert torch.equal(g != 0, y != 0) and d.rng_state[1] == 2
+
+
+# ---- Seq2Seq -----------------------------------------------------------------
+
+def test_translate_leaves_each_module_in_its_mode():
+    model = Seq2Seq(20, 20, 16, 1, rnn='attention', dropout=0.1)
+    model.encoder.eval()  # frozen
+    before = {name: m.training for name, m in model.named_modules()}
+    assert model.training and not model.encoder.dropout.training
+    model.translate(torch.tensor([[1, 2]]), 3)
+    assert {name: m.training for name, m in model.named_modules()} == before
+    with pytest.raises(IndexError):
+        model.translate(torch.tensor([[1, 99]]), 3)
+    assert {name: m.training for name, m in model.named_modules()} == before
