@@ -33,7 +33,8 @@ class LinearAttentionRNN(nn.Module):
     """``forward(x, state=None, lengths=None) -> (output, state)``.
 
     ``x`` is ``[batch, length, input_size]``; the state ``[num_layers, batch,
-    n_heads, d, d]`` in fp32 with ``d = hidden_size / n_heads`` (at most 128).
+    n_heads, d, d]`` in fp32 with ``d = hidden_size / n_heads`` (at most 128;
+    by default there are the fewest equal heads from ``hidden_size // 64`` on).
     ``lengths`` are those of a padded batch.  The heads' memories, after which
     a token's weight has fallen to 1/e, are spread from ``memory[0]`` to
     ``memory[1]`` tokens and are not learned.  Under autocast the sum of the
@@ -45,6 +46,12 @@ class LinearAttentionRNN(nn.Module):
         super().__init__()
         if n_heads is None:
             n_heads = max(1, hidden_size // 64)
+            while hidden_size % n_heads:
+                n_heads += 1
+            if n_heads > 1 and hidden_size // n_heads < 16:
+                raise ValueError('LinearAttentionRNN: {} units have no equal '
+                                 'heads of 16 to 128; n_heads has to be '
+                                 'given'.format(hidden_size))
         if hidden_size % n_heads or hidden_size // n_heads > 128:
             raise ValueError('LinearAttentionRNN: {} units in {} heads: equal '
                              'heads of at most 128 units'.format(hidden_size,

@@ -162,3 +162,24 @@ def test_translate_leaves_each_module_in_its_mode():
     with pytest.raises(IndexError):
         model.translate(torch.tensor([[1, 99]]), 3)
     assert {name: m.training for name, m in model.named_modules()} == before
+
+
+@pytest.mark.parametrize('units,heads', [
+    (200, 4), (250, 5), (500, 10), (1000, 20),  # no multiples of 64
+    (8, 1), (100, 1), (192, 3), (512, 8), (1024, 16)])
+def test_attention_rnn_chooses_heads_that_fit(units, heads):
+    rnn = links.LinearAttentionRNN(units, units)
+    assert (rnn.n_heads, rnn.head) == (heads, units // heads)
+    y, state = rnn(torch.randn(2, 3, units))
+    assert y.shape == (2, 3, units)
+    assert state.shape == (1, 2, heads, units // heads, units // heads)
+
+
+def test_seq2seq_of_any_units():
+    model = Seq2Seq(9, 9, 200, 1, rnn='attention')
+    ids = torch.tensor([[1, 2, 3]])
+    model(ids, ids, ids).backward()
+    # units without heads of a useful size are still refused
+    for units in (509, 262):
+        with pytest.raises(ValueError, match='n_heads'):
+            links.LinearAttentionRNN(8, units)
