@@ -139,8 +139,8 @@ class EncoderPart(nn.Module):
         self.comm = comm
         self.decoder_rank = decoder_rank
 
-    def forward(self, xs):
-        state = self.encoder(xs)
+    def forward(self, xs, lengths=None):
+        state = self.encoder(xs, lengths)
         state = state.contiguous() if isinstance(state, torch.Tensor) \
             else tuple(x.contiguous() for x in state)
         delegate = functions.send(state, self.comm, self.decoder_rank)

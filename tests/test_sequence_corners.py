@@ -5,8 +5,10 @@ import torch
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
+import chainermn_amd
 from chainermn_amd import functions, links
-from chainermn_amd.models.seq2seq import Seq2Seq
+from chainermn_amd.models.seq2seq import Seq2Seq, make_model_parallel
+from chainermn_amd.testing import run_distributed
 
 
 # ---- dropout that is computed again ------------------------------------------
@@ -183,3 +185,34 @@ def test_seq2seq_of_any_units():
     for units in (509, 262):
         with pytest.raises(ValueError, match='n_heads'):
             links.LinearAttentionRNN(8, units)
+
+
+def _padded_worker(rank, size):
+    comm = chainermn_amd.create_communicator('naive')
+    model, xs, ys, lengths = padded_batch()
+    part = make_model_parallel(model, comm, 0, 1)
+    if rank == 0:
+        part(xs, lengths).backward()
+        return {'g': model.encoder.embed.weight.grad}
+    loss = part(ys, ys)
+    loss.backward()
+    return {'loss': loss.detach(), 'g': model.decoder.embed.weight.grad}
+
+
+def padded_batch():
+    torch.manual_seed(1)
+    model = Seq2Seq(11, 13, 16, n_layers=2, rnn='attention')
+    return (model, torch.randint(0, 11, (3, 5)), torch.randint(0, 13, (3, 4)),
+            torch.tensor([5, 0, 2]))
+
+
+def test_a_padded_batch_split_over_ranks():
+    results = run_distributed(_padded_worker, 2)
+    model, xs, ys, lengths = padded_batch()
+    loss = model(xs, ys, ys, lengths)
+    loss.backward()
+    assert torch.allclose(torch.from_numpy(results[1]['loss']),
+                          loss.detach(), atol=1e-5)
+    for rank, part in enumerate((model.encoder, model.decoder)):
+        assert torch.allclose(torch.from_numpy(results[rank]['g']),
+                              part.embed.weight.grad, atol=1e-5)
