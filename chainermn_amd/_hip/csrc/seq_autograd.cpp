@@ -169,17 +169,18 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     if (!g[0].defined() && !g[1].defined())
       return {none, none, none, none, none, none, none};
     const Tensor go = g[0].defined() ? g[0] : at::zeros_like(s[2]);
+    const bool need_first = s[4].defined() && ctx->needs_input_grad(4);
     auto [gq, gk, gv, gfirst] = linear_attention_bwd(
         s[0], s[1], s[2], s[3], some(s[4]), some(s[5]),
         ctx->saved_data["scale"].toDouble(), s[6], go,
         g[1].defined() ? c10::optional<Tensor>(g[1].contiguous())
                        : c10::nullopt,
         ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-        ctx->needs_input_grad(2), s[4].defined() && ctx->needs_input_grad(4));
+        ctx->needs_input_grad(2), need_first);
     return {ctx->needs_input_grad(0) ? gq : none,
             ctx->needs_input_grad(1) ? gk : none,
             ctx->needs_input_grad(2) ? gv : none, none,
-            gfirst.numel() ? gfirst : none, none, none};
+            need_first ? gfirst : none, none, none};
   }
 };
 

@@ -80,6 +80,18 @@ def test_a_state_that_nothing_is_added_to_decays(t, length, rate):
     close(gk, want * lam[:-1].flip(0)[:, None, None], sums(dv), dv * least)
 
 
+@pytest.mark.parametrize('b,h', [(0, 2), (3, 0)])
+def test_gradients_of_no_sequences(b, h):
+    q = torch.empty(b, 5, h, 8, device=DEV, requires_grad=True)
+    v = torch.empty(b, 5, h, 4, device=DEV, requires_grad=True)
+    s0 = torch.empty(b, h, 8, 4, device=DEV, requires_grad=True)
+    o, s = functions.linear_attention(q, q, v, torch.zeros(h, device=DEV),
+                                      initial_state=s0)
+    for x, g in zip((q, v, s0), torch.autograd.grad(
+            (o, s), (q, v, s0), (torch.ones_like(o), torch.ones_like(s)))):
+        assert g.shape == x.shape and g.dtype == x.dtype
+
+
 # ---- dropout that is computed again ------------------------------------------
 
 def dropout_layers():
