@@ -34,20 +34,27 @@ def _mul(a, c):
     return (high + (low >> 16)) >> 16, (low + (high << 16)) & _M
 
 
-def philox_words(key, n):
-    """Words 0..n-1 (int64 below 2^32) of the Philox4x32-10 stream whose key
-    is ``key[0]`` and whose upper counter half is ``key[1]``."""
-    block = torch.arange((n + 3) // 4, device=key.device)
-    c0, c1 = block & _M, block >> 32
-    c2 = (key[1] & _M).expand_as(block)
-    c3 = ((key[1] >> 32) & _M).expand_as(block)
-    k0, k1 = key[0] & _M, (key[0] >> 32) & _M
+def philox(c0, c1, c2, c3, k0, k1):
+    """Philox4x32-10 of a counter and a key: words below 2^32, as whole
+    numbers or int64 tensors."""
     for _ in range(10):
         h0, l0 = _mul(0xD2511F53, c0)
         h1, l1 = _mul(0xCD9E8D57, c2)
         c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
         k0, k1 = (k0 + 0x9E3779B9) & _M, (k1 + 0xBB67AE85) & _M
-    return torch.stack((c0, c1, c2, c3), 1).reshape(-1)[:n]
+    return c0, c1, c2, c3
+
+
+def philox_words(key, n, block=0):
+    """Words 4 * block .. 4 * block + n - 1 (int64 below 2^32) of the
+    Philox4x32-10 stream whose key is ``key[0]`` and whose upper counter half
+    is ``key[1]``."""
+    block = torch.arange(block, block + (n + 3) // 4, device=key.device)
+    c2 = (key[1] & _M).expand_as(block)
+    c3 = ((key[1] >> 32) & _M).expand_as(block)
+    words = philox(block & _M, block >> 32, c2, c3, key[0] & _M,
+                   (key[0] >> 32) & _M)
+    return torch.stack(words, 1).reshape(-1)[:n]
 
 
 def dropout_plain(x, key, threshold, scale):

@@ -8,7 +8,44 @@ from torch.utils.checkpoint import checkpoint
 import chainermn_amd
 from chainermn_amd import functions, links
 from chainermn_amd.models.seq2seq import Seq2Seq, make_model_parallel
+from chainermn_amd.ops._dropout import philox, philox_words
 from chainermn_amd.testing import run_distributed
+
+
+# ---- the stream of dropout ---------------------------------------------------
+
+@pytest.mark.parametrize('counter,key,words', [
+    ((0,) * 4, (0,) * 2, '6627e8d5 e169c58d bc57ac4c 9b00dbd8'),
+    ((2 ** 32 - 1,) * 4, (2 ** 32 - 1,) * 2,
+     '408f276d 41c83b0e a20bc7c6 6d5451fd'),
+    ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344),
+     (0xa4093822, 0x299f31d0), 'd16cfe09 94fdcceb 5001e420 24126ea1')])
+def test_philox_published_vectors(counter, key, words):
+    # the numbers themselves, and by tensors
+    want = [int(w, 16) for w in words.split()]
+    assert list(philox(*counter, *key)) == want
+    assert [int(w) for w in philox(*(torch.tensor(x)
+                                     for x in counter + key))] == want
+    # the stream puts a block's number in front of the call's, each with its
+    # lower half first, and the seed into the key
+    def signed(low, high):
+        x = high << 32 | low
+        return x - 2 ** 64 if x >= 2 ** 63 else x
+    if counter[1] < 2 ** 31:  # a block's number is not negative
+        block = signed(*counter[:2])
+        assert philox_words(torch.tensor([signed(*key), signed(
+            *counter[2:])]), 4, block).tolist() == want
+
+
+def test_philox_words_of_all_halves():
+    seed, call, block = -0x123456789abcdef, 0x7edcba987654321f, 0x35a4e00000007
+    m = 2 ** 32 - 1
+    want = [list(philox(b & m, b >> 32, call & m, call >> 32, seed & m,
+                        (seed >> 32) & m)) for b in (block, block + 1)]
+    assert philox_words(torch.tensor([seed, call]), 8, block).tolist() == \
+        want[0] + want[1]
+    assert philox_words(torch.tensor([seed, call]), 5, block).tolist() == \
+        (want[0] + want[1])[:5]
 
 
 # ---- dropout that is computed again ------------------------------------------

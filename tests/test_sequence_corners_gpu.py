@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
     from chainermn_amd import functions, links
+    from chainermn_amd.ops._dropout import philox_words
     DEV = torch.device('cuda:0')
 else:
     pytest.skip('needs ROCm GPU', allow_module_level=True)
@@ -90,6 +91,57 @@ def test_gradients_of_no_sequences(b, h):
     for x, g in zip((q, v, s0), torch.autograd.grad(
             (o, s), (q, v, s0), (torch.ones_like(o), torch.ones_like(s)))):
         assert g.shape == x.shape and g.dtype == x.dtype
+
+
+# ---- the stream of dropout ---------------------------------------------------
+
+@pytest.mark.parametrize('seed,call', [
+    (5, 0), (-0x123456789abcdef, 0x7edcba987654321f)])
+def test_dropout_takes_all_halves_of_its_key(seed, call):
+    key = torch.tensor([seed, call])
+    kept = philox_words(key, 4003) >= 2 ** 31
+    y = functions.dropout(torch.ones(4003, device=DEV), key.to(DEV), 0.5)
+    assert torch.equal(y.cpu() != 0, kept)
+
+
+def test_dropout_past_2_32_blocks():
+    """2^34 elements and more: the block's number takes two words."""
+    n = 2 ** 34 + 4099
+    key = torch.tensor([0x1234567890abcdef, 3])
+    x = torch.ones(n, device=DEV, dtype=torch.bfloat16)
+    y = functions.dropout(x, key.to(DEV), ratio=0.5)
+    for block, size in ((0, 4096), (2 ** 32 - 1024, 8192 + 3)):
+        kept = philox_words(key, size, block) >= 2 ** 31
+        assert torch.equal((y[4 * block:4 * block + size] != 0).cpu(), kept)
+    del x, y
+    torch.cuda.empty_cache()
+
+
+# ---- what is changed between the passes --------------------------------------
+
+def test_inputs_changed_between_the_passes_are_seen():
+    """As for torch's own operators: an error, and no wrong gradient."""
+    ids = torch.arange(6, device=DEV)
+    key = torch.tensor([1, 2], device=DEV)
+    ld = torch.full((2,), -0.1, device=DEV)
+    w = rand(16)
+
+    def attend(x):
+        q = x.view(2, 3, 2, 8)
+        return functions.linear_attention(q, q, q, ld)[0]
+
+    for run, changed in [
+            (lambda x: functions.rms_norm(x, w), None),
+            (lambda x: functions.rms_norm(x.view(2, 3, 16), w, x.view(
+                2, 3, 16))[0], None),
+            (attend, None),
+            (lambda x: functions.embed_id(ids, x), ids),
+            (lambda x: functions.dropout(x, key), key)]:
+        x = rand(6, 16).requires_grad_() * 1
+        y = run(x)
+        (x if changed is None else changed).add_(1)
+        with pytest.raises(RuntimeError, match='inplace'):
+            y.sum().backward()
 
 
 # ---- dropout that is computed again ------------------------------------------
