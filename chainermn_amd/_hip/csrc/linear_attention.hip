@@ -39,13 +39,19 @@
 //
 // All products run on bf16 matrix instructions (16x16x32) with fp32 sums:
 // a value is cut into terms of 8 bits of mantissa each, exactly: bf16 is one
-// term, fp16 two, fp32 three, and products of terms below 2^-24 of the
-// largest (2^-16 where the result is rounded to 16 bits) are left out.  The
-// state is fp32 throughout, and what is added to it is a product of three
-// terms.  The contraction index of a matrix instruction may be permuted if
-// both operands are, so that the accumulators of the state and the scores
-// (four consecutive rows for a lane) are operands of the next product as
-// they stand: lane group g holds 4g..4g+3 and 16+4g..16+4g+3 of 32.
+// term, fp16 two, fp32 three.  They are cut off, not rounded, so the second
+// is below 2^-7 of the first one's power of two and the third below 2^-15.  Of
+// a product of three terms each, those of second with third and of third with
+// third terms are left out, less than 2^-21 of it.  A result that is itself
+// rounded to 16 bits, by up to 2^-11 (fp16) or 2^-8 (bf16), takes scores and
+// states with two terms (2^-15), and leaves out second with second terms
+// (2^-14, fp16 only).  What is left out has the sign of the product.  The state
+// is fp32 throughout, and what is added to it is a product of three terms.
+//
+// The contraction index of a matrix instruction may be permuted if both
+// operands are, so that the accumulators of the state and the scores (four
+// consecutive rows for a lane) are operands of the next product as they
+// stand: lane group g holds 4g..4g+3 and 16+4g..16+4g+3 of 32.
 
 #include "seq_common.h"
 

@@ -81,6 +81,29 @@ def test_a_state_that_nothing_is_added_to_decays(t, length, rate):
     close(gk, want * lam[:-1].flip(0)[:, None, None], sums(dv), dv * least)
 
 
+def test_products_of_terms_at_their_worst():
+    """Numbers whose three terms of eight bits are as large as they can be.
+
+    Of a number 2^e (1 + ..) the second term is below 2^-7 2^e and the third
+    below 2^-15 2^e.  The products that are left out, of second with third and
+    third with third terms, are below 2^-21 of the product, and the one sum of
+    its size is off by at most 2^-23.  An output is two such products after
+    each other and a factor, the state one."""
+    worst = 1 + 2.0 ** -7 - 2.0 ** -23
+    g = torch.Generator().manual_seed(0)
+    sign = torch.randint(0, 2, (3, 64, 1, 1, 1), generator=g) * 2.0 - 1
+    power = 2.0 ** torch.randint(-9, 9, (3, 64, 1, 1, 1), generator=g)
+    q, k, v = (worst * sign * power).to(DEV)
+    o, s = functions.linear_attention(q, k, v, torch.zeros(1, device=DEV),
+                                      scale=1.0)
+    q, k, v = q.double(), k.double(), v.double()
+    for got, want, bound in (
+            (o, q * k * v, 2 * (2.0 ** -21 + 2.0 ** -23) + 2 * E),
+            (s, k * v, 2.0 ** -21 + 2.0 ** -23 + E)):
+        off = (got.double() - want).abs() / want.abs()
+        assert float(off.max()) <= bound
+
+
 @pytest.mark.parametrize('b,h', [(0, 2), (3, 0)])
 def test_gradients_of_no_sequences(b, h):
     q = torch.empty(b, 5, h, 8, device=DEV, requires_grad=True)
