@@ -12,7 +12,7 @@
 //
 // Bound by memory: one read and one write of each element.  A 32 x 32 bit
 // product is one instruction here, so ten rounds for four elements stay below
-// that.  2^27 elements of bf16: 104 us, 5.2 TB/s (a large copy reaches 4.9).
+// that.  2^27 elements of bf16: 97 us, 5.6 TB/s (torch's copy reaches 4.9).
 
 #include "seq_common.h"
 

@@ -3,9 +3,10 @@
 //   y[t]  = c * W[id_t]                       (zero where id_t is ignored)
 //   dW[v] = c * sum of gy[t] over id_t == v   (the whole table, zeros too)
 //
-// Both are bound by memory.  32768 tokens of 32000 x 1024 in fp32: the lookup
-// takes 39 us, 5 TB/s of what it has to move, and the gradient 80 us: 55 us
-// for embed_rows, 4.8 TB/s, 18 us for the order and 7 us for embed_join.
+// 32768 tokens of 32000 x 1024 in fp32, 8791 rows of them: the lookup takes 38
+// us, 4.5 TB/s of what it has to move, and the gradient 81 us: 55 us for
+// embed_rows, 4.8 TB/s, which memory bounds, 18 us for the order and 7 us for
+// embed_join, which latency does, with memory idle.
 // (With one sorting pass, in which every workgroup reads all ids, the order
 // alone took 50 us.)
 //
@@ -19,11 +20,14 @@
 //      for another one.  Low bits, because the frequent words of a vocabulary
 //      sorted by frequency are neighbours.  16 waves: the bucket of the most
 //      frequent word lasts longest.  (262144 tokens, 7% of them one word, both
-//      passes: 402 us; with 8 waves 429 us.)
+//      passes: 402 us; with 8 waves 429 us.)  A bucket's
+//      workgroup sorts a frequent word alone: where half of 32768 tokens are
+//      one word, the gradient takes 112 us instead of 64 us (the same input
+//      again and again, in the caches), so padding should be ignored.
 //   2. embed_rows: a wave sums 8 to 32 sorted tokens of some columns; rows
 //      that begin and end within its tokens are finished, the two at its
 //      ends leave partial sums.  So a frequent word costs no more than
-//      others.  Rows without a token are zeroed by further waves.
+//      others here.  Rows without a token are zeroed by further waves.
 //   3. embed_join: adds up the partial sums of rows that span chunks.
 
 #include "seq_common.h"
@@ -573,9 +577,12 @@ torch::Tensor embed_grad(torch::Tensor ids, torch::Tensor gy, long vocab,
   auto dw = torch::empty({vocab, dim}, gy.options());
   const int ve = 16 / (int)gy.element_size();
   const int slices = int((dim + 64 * ve - 1) / (64 * ve));
-  // A row of the table for each workgroup, while there are no more than run
-  // at once and no more tokens than a wave finds quickly.  (1280 tokens of 64
-  // x 512 in fp32: 5 us instead of 22 us.)
+  // A row of the table for each workgroup, while they are two rounds of this
+  // GPU at most and there are no more tokens than a wave finds quickly.  (1280
+  // tokens: 512 rows of 256 in fp32 5 us, by the sort 22 us; 256 rows of 1024 6
+  // us, 21 us.  4096 tokens, 1024 rows of 256: 7 us, 23 us, and 4096 rows 17
+  // us, 23 us; 16 rows of 1024 15 us, 24 us.  Only one word is the worst, since
+  // its row's workgroup sums all of it: 4096 tokens 45 us.)
   if (vocab * slices <= 1024 && n <= 4096) {
     dispatch(gy.scalar_type(), "embed_grad", [&](auto t) {
       using T = decltype(t);

@@ -26,12 +26,15 @@
 // bf16: 381 us with 32, 443 us with 64).  A wave has 16 columns of the state;
 // with 32 the same took 388 us instead of 348 us.
 //
-// What bounds it: for heads of 64 the memory (512 x 64 tokens, 16 heads, fp32:
-// forward 111 us, 6 TB/s, backward 255 us); for heads of 128 in bf16 the
-// instructions of a chunk, whose phases lie between three barriers (128 x 512
-// tokens, 4 heads: forward 71 us, 4.3 TB/s, 62 us with all inputs in L2;
-// backward 190 us).  2 x 16384 tokens, 8 heads: forward 114 us, of which
-// states of segments and joining them 40 us; backward 240 us.
+// What bounds it: forward the memory, where there are many heads of 64 (512 x
+// 64 tokens, 16 heads, fp32: 144 us, 4.7 TB/s of what it has to move; with half
+// of the tokens there 111 us, 4.3 TB/s).  Otherwise the instructions of a
+// chunk, whose phases lie between three barriers: backward of the same 310 us
+// and 257 us, 3.0 and 2.6 TB/s, vector pipes 52% and LDS 40% busy; 128 x 512
+// tokens, 4 heads of 128 in bf16, 75 us and 187 us.  2 x 16384 tokens, 8 heads
+// of 128: forward 117 us, of which states of segments and joining them 40 us;
+// backward 241 us.  (Pairs of figures for a choice were taken side by side,
+// with the rest as it was then, and may differ from these.)
 //
 // Long sequences and few heads: the length is cut into segments.  The states
 // of the segments alone come first, a scan joins them, and the same kernel
@@ -45,8 +48,10 @@
 // third terms are left out, less than 2^-21 of it.  A result that is itself
 // rounded to 16 bits, by up to 2^-11 (fp16) or 2^-8 (bf16), takes scores and
 // states with two terms (2^-15), and leaves out second with second terms
-// (2^-14, fp16 only).  What is left out has the sign of the product.  The state
-// is fp32 throughout, and what is added to it is a product of three terms.
+// (2^-14, fp16 only).  What is left out has the sign of the product.  A term
+// below 2^-126 counts as zero, so that fp32 values below 2^-110 have fewer bits.
+// The state is fp32 throughout, and what is added to it is a product of three
+// terms.
 //
 // The contraction index of a matrix instruction may be permuted if both
 // operands are, so that the accumulators of the state and the scores (four
@@ -1165,6 +1170,8 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
   if (b * h == 0) return o;
   check_grid(b * h, kThreads, "linear_attention_step");
   state.unsafeGetTensorImpl()->bump_version();
+  // rows of other lengths by elements: heads of 63 take 8.6 us where 64 take
+  // 6.5 us, of 127 42 us where 128 take 22 us (64 sequences, 16 heads, bf16)
   const bool wide = dv % 4 == 0;
   dispatch(q.scalar_type(), "linear_attention_step", [&](auto t) {
     using T = decltype(t);

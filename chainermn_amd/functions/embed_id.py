@@ -10,9 +10,11 @@ def embed_id(x, W, ignore_label=None, scale=1.0):
     ``x.shape + (units,)`` in W's type.
 
     An id equal to ``ignore_label`` (any number, -1 or 0 for instance) gives
-    a row of zeros and no gradient.  Any other id outside of the vocabulary
-    is an error: an IndexError on the CPU; on the GPU, where finding out would
-    stop the stream, its row is NaN and has no gradient.
+    a row of zeros and no gradient.  Padding should be such an id: one that
+    is looked up is summed like a word, more slowly the more of it there is.
+    Any other id outside of the vocabulary is an error: an IndexError on the
+    CPU; on the GPU, where finding out would stop the stream, its row is NaN
+    and has no gradient.
 
     The gradient of W is dense.  It is summed in fp32 in the order of the
     tokens, without atomics: two runs agree bit by bit.

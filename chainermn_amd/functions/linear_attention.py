@@ -21,7 +21,8 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None,
     token.
 
     Returns ``(o, state)``: ``o`` like v, and the fp32 state behind the
-    sequences.  States and sums are fp32 whatever the type of q.  A value
+    sequences.  States and sums are fp32 whatever the type of q; products
+    of fp32 are good to 2^-21, and of values below 2^-110 less so.  A value
     that is not finite spreads to the outputs of its own chunk of 32 tokens,
     those before it included.
     """
