@@ -796,7 +796,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Problem pr,
 }
 
 // One token: the state is read, updated in place and written, and bounds the
-// kernel (64 sequences, 16 heads of 64: 7.4 us, 4.6 TB/s).  A workgroup has
+// kernel (64 sequences, 16 heads of 64: 7.8 us, 4.4 TB/s).  A workgroup has
 // 16 * VE columns of the state of a sequence and head; a thread has VE of
 // them in every 16th row.
 template <typename T, int VE>
@@ -815,7 +815,11 @@ __global__ __launch_bounds__(kThreads) void step_kernel(
     const int i = t - 128;
     sk[i] = i < dk ? float(k[b * kb + h * kh + i]) : 0.f;
   }
-  const float lam = expf(log_decay[h]);
+  // as in the chunks: a state of a long memory changes by what it forgets
+  Decay decay;
+  decay.set(log_decay[h], 1);
+  const bool near = decay.far == 1.f;
+  const float by = near ? decay.by : decay.far;
   const int c = (blockIdx.y * 16 + (t & 15)) * VE;
   const bool on = c < dv;
   float* s = state + (long)bh * dk * dv + c;
@@ -833,7 +837,8 @@ __global__ __launch_bounds__(kThreads) void step_kernel(
       load<float, VE>(s + (long)i * dv, r);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        r[e] = r[e] * lam + sk[i] * x[e];
+        r[e] = __builtin_fmaf(r[e], by,
+                              __builtin_fmaf(sk[i], x[e], near ? r[e] : 0.f));
         acc[e] += sq[i] * r[e];
       }
       store<float, VE>(s + (long)i * dv, r);
@@ -1170,8 +1175,9 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k,
   if (b * h == 0) return o;
   check_grid(b * h, kThreads, "linear_attention_step");
   state.unsafeGetTensorImpl()->bump_version();
-  // rows of other lengths by elements: heads of 63 take 8.6 us where 64 take
-  // 6.5 us, of 127 42 us where 128 take 22 us (64 sequences, 16 heads, bf16)
+  // rows of other lengths by elements: heads of 63 take 8.7 us where 64 take
+  // 6.8 us, of 127 43 us where 128 take 23 us (64 sequences, 16 heads, bf16,
+  // by a graph)
   const bool wide = dv % 4 == 0;
   dispatch(q.scalar_type(), "linear_attention_step", [&](auto t) {
     using T = decltype(t);

@@ -98,6 +98,7 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None):
             q, k, v, state, log_decay.contiguous(), float(scale))
     if not state.is_contiguous():
         raise ValueError('linear_attention: a state is contiguous')
-    state.mul_(torch.exp(log_decay)[:, None, None]).add_(
-        k.float()[..., None] * v.float()[..., None, :])
+    # in fp64: rounded, a decay near one would lose what a long memory forgets
+    state.copy_(state.double() * torch.exp(log_decay.double())[:, None, None]
+                + k.double()[..., None] * v.double()[..., None, :])
     return ((q.float()[..., None] * state).sum(-2) * scale).to(q.dtype)

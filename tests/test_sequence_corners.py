@@ -6,7 +6,7 @@ import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
 import chainermn_amd
-from chainermn_amd import functions, links
+from chainermn_amd import functions, links, ops
 from chainermn_amd.models.seq2seq import Seq2Seq, make_model_parallel
 from chainermn_amd.ops._dropout import philox, philox_words
 from chainermn_amd.testing import run_distributed
@@ -187,6 +187,21 @@ def test_a_forgotten_segment_that_fails():
     y = functions.forget(lambda t: d(t) * t, x)
     g, = torch.autograd.grad(y.sum(), x)
     assert torch.equal(g != 0, y != 0) and d.rng_state[1] == 2
+
+
+# ---- single tokens -----------------------------------------------------------
+
+def test_single_tokens_keep_a_long_memory():
+    # a rounded decay would be off by 2^-25 in each step, the same way for all
+    ld = torch.tensor([-1 / 3e4, -1 / 4096])
+    state = torch.rand(1, 2, 64, 64) + 0.5
+    zero = torch.zeros(1, 2, 64)
+    want = state.double() * torch.exp(2000 * ld.double())[:, None, None]
+    for _ in range(2000):
+        ops.linear_attention_step(zero, zero, zero, state, ld)
+    mean = ((state.double() - want) / want).mean((0, 2, 3))
+    # 2000 roundings that cancel over 4096 elements: a spread of 45 E / 64
+    assert float(mean.abs().max()) <= 8 * 2.0 ** -24
 
 
 # ---- Seq2Seq -----------------------------------------------------------------

@@ -11,7 +11,7 @@ from torch.utils.checkpoint import checkpoint
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
-    from chainermn_amd import functions, links
+    from chainermn_amd import functions, links, ops
     from chainermn_amd.ops._dropout import philox_words
     DEV = torch.device('cuda:0')
 else:
@@ -102,6 +102,43 @@ def test_products_of_terms_at_their_worst():
             (s, k * v, 2.0 ** -21 + 2.0 ** -23 + E)):
         off = (got.double() - want).abs() / want.abs()
         assert float(off.max()) <= bound
+
+
+@pytest.mark.parametrize('dv', [64, 61])
+def test_single_tokens_forget_as_the_chunks_do(dv):
+    """4096 tokens that add nothing: each element takes 4096 roundings of up
+    to E, which cancel over the elements (a mean of 16 * 64 * dv of them, each
+    of a spread of 64 E at most, is off by less than E).  What is forgotten in
+    a step is off by 2 E of itself, 2 * 4096 / memory E in all.  A rounded decay
+    would be off by up to E / 2 in each step, the same way for all."""
+    memories = torch.tensor([8.0, 200.0, 4096.0, 7000.0, 30000.0], device=DEV)
+    ld = -1 / memories
+    h = len(ld)
+    state, zero = rand(16, h, 64, dv), torch.zeros(16, h, 64, device=DEV)
+    none = torch.zeros(16, h, dv, device=DEV)
+    want = state.double() * torch.exp(4096 * ld.double())[:, None, None]
+    tokens = torch.zeros(16, 4096, h, 64, device=DEV)
+    _, chunked = functions.linear_attention(
+        tokens, tokens, tokens[..., :dv], ld, initial_state=state)
+    for _ in range(4096):
+        ops.linear_attention_step(zero, zero, none, state, ld)
+    for got in (state, chunked):
+        mean = ((got.double() - want) / want)[:, 1:].mean((0, 2, 3))
+        assert bool((mean.abs() <= (16 + 8192 / memories[1:]) * E).all()), mean
+    # exp(-512); in steps of 2^-149 the rounding of m exp(-1/8) ends at an m of
+    # four, since four times 1 - exp(-1/8) is below a half
+    assert float(state[:, 0].max()) <= 4 * 2.0 ** -149
+
+
+def test_a_single_token_of_extreme_decays():
+    ld = torch.tensor([float('-inf'), 0.0, -1000.0, -0.7, -0.69], device=DEV)
+    state, q = rand(2, 5, 8, 6, seed=1), rand(2, 5, 8)
+    k, v = rand(2, 5, 8, seed=2), rand(2, 5, 6, seed=3)
+    new = torch.einsum('bhi,bhj->bhij', k.double(), v.double())
+    want = state.double() * torch.exp(ld.double())[:, None, None] + new
+    o = ops.linear_attention_step(q, k, v, state, ld, scale=1.0)
+    close(state, want, 3 * E, 0.0)  # all positive
+    close(o, torch.einsum('bhi,bhij->bhj', q.double(), want), 14 * E, 0.0)
 
 
 @pytest.mark.parametrize('b,h', [(0, 2), (3, 0)])
